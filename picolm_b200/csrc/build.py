@@ -41,6 +41,8 @@ LIBRARIES: Dict[str, List[str]] = {
     "attention_simt": ["attention_simt.cu"],
     "attention_mma": ["attention_mma.cu"],          # one variant per head size: "attention_mma@hd64" with -DPLM_HD=64
     "attention_tc": ["attention_tc.cu"],            # likewise, head sizes 64 and 128
+    "kv8": ["kv8.cu"],
+    "attention_kv8": ["attention_kv8.cu"],          # one variant per head size, as attention_mma
     "sampling": ["sampling.cu"],
     "recurrent": ["recurrent.cu"],
     "routed": ["routed.cu"],
@@ -51,13 +53,14 @@ LIBRARIES: Dict[str, List[str]] = {
     "delta_chunk": ["delta_chunk.cu"],
     "scan_chunk": ["scan_chunk.cu"],
 }
-HEADERS = ["common.cuh", "tc_common.cuh", "split_common.cuh", "mma_common.cuh", "gemm_tc_static.h"]
+HEADERS = ["common.cuh", "tc_common.cuh", "split_common.cuh", "mma_common.cuh", "kv8.cuh", "gemm_tc_static.h"]
 
 # Libraries that are specialised at compile time.  At run time only the variant a
 # model needs is built (`attention_variant`); the build check builds these.
 VARIANTS: Dict[str, Dict[str, List[str]]] = {
     "attention_mma": {f"hd{hd}": [f"-DPLM_HD={hd}"] for hd in (64, 128)},
     "attention_tc": {f"hd{hd}": [f"-DPLM_HD={hd}"] for hd in (64, 128)},
+    "attention_kv8": {f"hd{hd}": [f"-DPLM_HD={hd}"] for hd in (64, 128)},
 }
 
 

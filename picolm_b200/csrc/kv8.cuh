@@ -1,0 +1,88 @@
+// What the kernels of the 8-bit cache share.
+//
+// The format.  Keys and values are e4m3 numbers [pages, G, 64, hd] with one scale for each page and kv head, float32
+// [pages, G], a power of two 2^e with KV8_E_MIN <= e <= KV8_E_MAX: the smallest with 448 * 2^e at or above the largest
+// finite magnitude that the page holds (448 is e4m3's largest number).  What a place holds is number * scale; a value that is not finite
+// is held as NaN, one beyond 448 * 2^KV8_E_MAX as that.  With scales that are powers of two a page whose scale has to grow
+// keeps what it holds: its numbers' exponents shift, and only those that become subnormal (below 2^-6) are rounded again.
+// The bounds of e keep 2^(e - e') of any two pages and sums in the unit of either inside float32.
+#pragma once
+#include "common.cuh"
+#include <cuda_fp16.h>
+
+constexpr int KV8_E_MIN = -60, KV8_E_MAX = 40;
+
+// Two e4m3 numbers, the low byte's first, as halves (exact; NaN stays NaN).
+__device__ __forceinline__ uint32_t kv8_halves(uint32_t two) {
+    uint32_t r;
+    asm("{\n\t.reg .b16 h;\n\tcvt.u16.u32 h, %1;\n\tcvt.rn.f16x2.e4m3x2 %0, h;\n\t}" : "=r"(r) : "r"(two));
+    return r;
+}
+__device__ __forceinline__ float2 kv8_floats(uint32_t two) {
+    const uint32_t h = kv8_halves(two);
+    return __half22float2(*reinterpret_cast<const __half2*>(&h));
+}
+// Two floats as e4m3, to the nearest (ties to even), magnitudes above 448 held there; `a` in the low byte.
+__device__ __forceinline__ uint32_t kv8_pack(float a, float b) {
+    uint16_t r;
+    asm("cvt.rn.satfinite.e4m3x2.f32 %0, %2, %1;" : "=h"(r) : "f"(a), "f"(b));
+    return r;
+}
+// Infinity and NaN as NaN.
+__device__ __forceinline__ float kv8_finite_or_nan(float x) { return fabsf(x) < INFINITY ? x : __int_as_float(0x7fffffff); }
+// |x|, and 0 for what is not finite
+__device__ __forceinline__ float kv8_magnitude(float x) {
+    const float a = fabsf(x);
+    return a < INFINITY ? a : 0.f;
+}
+// The exponent of the scale for a largest magnitude: a = 1.f * 2^E <= 448 * 2^e = 1.75 * 2^(8 + e).
+__device__ __forceinline__ int kv8_exponent(float a) {
+    const uint32_t bits = __float_as_uint(a);
+    const int e = (int)(bits >> 23) - 127 - 8 + ((bits & 0x7fffffu) > 0x600000u ? 1 : 0);
+    return min(max(e, KV8_E_MIN), KV8_E_MAX);
+}
+__device__ __forceinline__ float kv8_pow2(int e) { return __int_as_float((e + 127) << 23); }      // -126 <= e <= 127
+__device__ __forceinline__ int kv8_exponent_of_scale(float s) { return (int)(__float_as_uint(s) >> 23) - 127; }
+
+// A step's sequence as attention sees it.  With tok_pos every row of q is a token of its own (`b` is its number), at
+// position tok_pos[b] of the sequence whose pages are row tok_seq[b] of the table; otherwise `b` is a sequence of the step,
+// its new tokens are rows seq_start[b] .. seq_start[b + 1] and its keys 0 .. seq_kv_len[b] - 1.
+struct Kv8Step {
+    const int *tok_pos, *tok_seq, *seq_start, *seq_kv_len, *block_table;
+    int max_pages;
+};
+struct Kv8Seq {
+    int t0, n_new, pos0;                     // first row of q, rows, position of the first
+    const int* pages;
+};
+__device__ __forceinline__ Kv8Seq kv8_seq(const Kv8Step& s, int b) {
+    Kv8Seq q;
+    if (s.tok_pos) {
+        q.t0 = b;
+        q.n_new = 1;
+        q.pos0 = PLM_POSITION(s.tok_pos[b]);
+        q.pages = s.block_table + (size_t)PLM_SEQ_NO(s.tok_seq[b]) * s.max_pages;
+    } else {
+        q.t0 = s.seq_start[b];
+        q.n_new = s.seq_start[b + 1] - q.t0;
+        q.pos0 = PLM_POSITION(s.seq_kv_len[b] - 1) + 1 - q.n_new;
+        q.pages = s.block_table + (size_t)b * s.max_pages;
+    }
+    return q;
+}
+
+// A row of q in front of the first sequence's or behind the last one's: no kernel looks at it or writes its result.
+__device__ __forceinline__ bool kv8_of_no_sequence(int row, const int* seq_start, int n_seqs) {
+    return seq_start && (row < seq_start[0] || row >= seq_start[n_seqs]);
+}
+
+// With a sink (one more term exp(sink) in the denominator) the factor that turns a row's sum_j exp2(s_j - m) v_j into its
+// result: 1 / (l + exp2(sink log2e - m)), written so that a sink far above the scores does not overflow.
+__device__ __forceinline__ float kv8_inverse(float m, float l, const float* sink) {
+    if (m == -INFINITY) return 0.f;
+    if (!sink) return 1.f / l;
+    const float sk = *sink * 1.4426950408889634f;
+    if (sk <= m) return 1.f / (l + exp2f(sk - m));
+    const float c = exp2f(m - sk);
+    return c / fmaf(l, c, 1.f);
+}

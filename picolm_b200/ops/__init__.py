@@ -16,6 +16,8 @@ from .elementwise import (GATE_ACTIVATIONS, add_bias, add_rows, dyt_norm, embed,
 from .gemm import (PLAIN_ACTIVATIONS, PendingLinear, ScaledRows, gemm_f32_tc, gemm_simt, gemm_tc_skinny, gemm_tc_supported,  # noqa: F401
                    gemm_tc_wide, interleave_gate_up, linear, linear_act, linear_residual_norm, linear_swiglu, pair_pays,
                    residual_norm_supported)
+from .kv8 import (KV8_DTYPE, attention_kv8_decode, attention_kv8_mma_supported, attention_kv8_prefill, kv8_supported,  # noqa: F401
+                  rope_store_kv8, store_kv8)
 from .recurrent import (IN_CHUNKS, ONE_PASS, SCAN_CHUNK_KEYS, StepShape, delta_scan_in_chunks, linear_scan_route, step_shape,  # noqa: F401
                         DECAY_CONST, DECAY_SIGMOID, DECAY_STEP, GATE_AFTER_NORM, GATE_BEFORE_NORM, GATE_NONE, causal_conv,  # noqa: F401
                         decay_chunk_supported, decay_in_128, decay_in_128_supported, decay_powers, decay_scan, delta_head_chunk_sizes, delta_prep, delta_scan, diag_scan, gated_norm, head_linear, linear_scan, rglru_gates,

@@ -102,6 +102,10 @@ _SIGNATURES = {
     "plm_gated_norm": [_vp, _i, _l, _vp, _i, _l, _vp, _i, _vp, _i, _l, _i, _i, _i, _f, _i, _i, _i, _vp],
     "plm_head_linear": [_vp, _i, _l, _vp, _vp, _i, _l, _vp, _l, _i, _i, _i, _i, _i, _vp],
     "plm_store_rows_paged": [_vp, _i, _l, _vp, _vp, _vp, _vp, _i, _i, _i, _vp],
+    "plm_kv8_append": [_vp, _vp, _vp, _i, _l, _l, _l, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _i, _vp, _vp, _vp, _i, _i, _i, _i, _i, _i, _i, _i, _vp],
+    "plm_kv8_attention_rows": [_vp, _i, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _i, _i, _i, _i, _i, _i, _i, _f, _i, _i, _vp, _i, _vp, _vp],
+    "plm_kv8_attention_few": [_vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _i, _i, _i, _i, _i, _i, _f, _i, _i, _vp, _i, _vp, _vp],
+    "plm_kv8_attention_tiles": [_vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _i, _i, _i, _i, _i, _f, _i, _vp, _i, _vp, _vp],
     "plm_argmax": [_vp, _l, _i, _i, _vp, _vp],
     "plm_sample": [_vp, _l, _i, _i, _f, _i, _f, _f, _vp, _vp, _vp],
 }
@@ -112,7 +116,7 @@ _fn_cache = {}
 # this package hand them the bounds before every launch.  An index outside its bound is then recorded in
 # the status word (`check_status` raises) instead of being followed.
 CHECKED = os.environ.get("PICOLM_B200_CHECK", "") == "1"
-CHECKED_LIBRARIES = ("elementwise", "attention_simt", "attention_mma", "attention_tc", "recurrent")
+CHECKED_LIBRARIES = ("elementwise", "attention_simt", "attention_mma", "attention_tc", "recurrent", "kv8", "attention_kv8")
 
 
 class KernelError(RuntimeError):
