@@ -11,13 +11,14 @@
 //
 // Two kernels:
 //   kv8_stream_kernel  few (token, head) rows a sequence and kv head, above all single tokens: bound by the cache's bytes.  A warp
-//                      walks a range of the keys on its own, 16 or 32 at a time, from global memory straight into the fragments
-//                      of its MMAs: no shared memory, no barrier on the way.  The keys are on the MMA's 16 rows and the
+//                      walks keys on its own, 16 or 32 at a time, through a ring of its own in shared memory (cp.async; no
+//                      barrier but the warp's).  The keys are on the MMA's 16 rows and the
 //                      (token, head) rows on its 8 columns, so that a group of four or eight heads does not leave half of the
 //                      MMA empty: S^T = K Q^T, and out^T = V^T P^T, whose A operand takes pairs of keys a component; a
 //                      byte permutation and a conversion make it of four rows of V.  The 8 columns of S^T become the
-//                      B operand by movmatrix.  Four warps' partial results meet in shared memory, up to eight CTAs' in
-//                      their cluster's, more through a workspace and a second kernel.
+//                      B operand by movmatrix.  Four warps' partial results meet in shared memory; CTAs' in their cluster's
+//                      where a step is small, else through a workspace and a second kernel, all keys of a step being dealt
+//                      out evenly over one wave of CTAs.
 //   kv8_tile_kernel    prompts of head sizes that the tcgen05 kernel does not take: 64 rows a CTA, pages of 64 keys brought to
 //                      shared memory as halves.
 #include "kv8.cuh"
@@ -34,8 +35,6 @@ constexpr float LOG2E = 1.4426950408889634f;
 constexpr int KS = HD / 16;                      // steps of the contraction over a head, and words of a key's row in a lane
 constexpr int MT = HD / 16;                      // tiles of 16 components
 constexpr int VW = (HD / 8 + 3) / 4;             // words of a value's row in a lane
-constexpr int SB = HD <= 64 ? 2 : 1;             // blocks of 16 keys that a warp works on at a time
-constexpr int KB = 16 * SB, UNITS = PLM_PAGE / KB;
 constexpr int WARPS = 4, NT = 128;
 constexpr float RAISE = 8.f;                     // a row's maximum may outgrow its reference by 2^RAISE before sums are scaled
 constexpr int UNIT_SPAN = 6;                     // weights take a page's unit up to 2^6 from the sums'
@@ -86,19 +85,6 @@ __device__ __forceinline__ int key_component(int w, int c) {
     if (B && w < 4 * A + 2) return 64 * A + c * 8 + (w - 4 * A) * 4;
     return 64 * A + 32 * B + c * 4;
 }
-__device__ __forceinline__ void load_key(uint32_t (&w)[KS], const uint8_t* row, int c) {
-    constexpr int A = HD / 64, B = (HD / 32) & 1, C = (HD / 16) & 1;
-#pragma unroll
-    for (int i = 0; i < A; ++i) {
-        const uint4 v = *reinterpret_cast<const uint4*>(row + i * 64 + c * 16);
-        w[4 * i] = v.x; w[4 * i + 1] = v.y; w[4 * i + 2] = v.z; w[4 * i + 3] = v.w;
-    }
-    if (B) {
-        const uint2 v = *reinterpret_cast<const uint2*>(row + 64 * A + c * 8);
-        w[4 * A] = v.x; w[4 * A + B] = v.y;
-    }
-    if (C) w[KS - 1] = *reinterpret_cast<const uint32_t*>(row + 64 * A + 32 * B + c * 4);
-}
 // A value's row in the eight lanes (n = lane / 4) that share it: bytes 2 m and 2 m + 1 of a lane are its components of the
 // m-th tile: rows n and n + 8 of the MMA.
 __device__ __forceinline__ int value_component(int m, int n) {
@@ -108,20 +94,80 @@ __device__ __forceinline__ int value_component(int m, int n) {
     if (C && m < 8 * A + 4 * B + 2) return 128 * A + 64 * B + n * 4 + (m - 8 * A - 4 * B) * 2;
     return 128 * A + 64 * B + 32 * C + n * 2;
 }
-__device__ __forceinline__ void load_value(uint32_t (&w)[VW], const uint8_t* row, int n) {
-    constexpr int A = HD / 128, B = (HD / 64) & 1, C = (HD / 32) & 1, D = (HD / 16) & 1;
+// Rows as they lie in shared memory: 16-byte chunk j of row r.  For heads of 64 and of multiples of 128 the chunks of a 128-byte line
+// change places by the row, so that the lanes of the loads below (rows n for keys, 2 c for values) find 32 banks.
+__device__ __forceinline__ uint32_t key_chunk(int r, int j) {
+    if constexpr (HD == 64) return (r >> 1) * 128 + ((((r & 1) * 4 + j) ^ (((r >> 1) & 3) * 2)) << 4);
+    else if constexpr (HD % 128 == 0) return r * HD + (j >> 3) * 128 + (((j & 7) ^ ((r & 1) * 4)) << 4);
+    else return r * HD + j * 16;
+}
+__device__ __forceinline__ uint32_t value_chunk(int r, int j) {
+    if constexpr (HD == 64) return key_chunk(r, j);
+    else if constexpr (HD % 128 == 0) return r * HD + (j >> 3) * 128 + (((j & 7) ^ (((r >> 1) & 3) * 2)) << 4);
+    else return r * HD + j * 16;
+}
+// The same as a lane's place and constants: chunk 32 x + lane of a tile lies at key_place / value_place of `at` = the chunk
+// function of chunk `lane`.  (Eight rows further on the places are the same, and 32 chunks are 8, 4 or 2 rows.)
+__device__ __forceinline__ uint32_t key_place(uint32_t at, int x) { return at + x * 512; }
+__device__ __forceinline__ uint32_t value_place(uint32_t at, int x) {
+    return (HD == 128 ? at ^ ((x & 1) * 64) : HD == 256 ? at ^ ((x & 3) * 32) : at) + x * 512;
+}
+template <typename T> __device__ __forceinline__ T lds(uint32_t at) {
+    T v;
+    if constexpr (sizeof(T) == 16)
+        asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(at) : "memory");
+    else if constexpr (sizeof(T) == 8)
+        asm volatile("ld.shared.v2.u32 {%0, %1}, [%2];" : "=r"(v.x), "=r"(v.y) : "r"(at) : "memory");
+    else
+        asm volatile("ld.shared.u32 %0, [%1];" : "=r"(v) : "r"(at) : "memory");
+    return v;
+}
+// Row n of eight at shared-memory address `rows`; at = key_chunk(n, c).  (The places of row n + 8 i are 8 HD i further on.)
+__device__ __forceinline__ void load_key(uint32_t (&w)[KS], uint32_t rows, uint32_t at, int n, int c) {
+    constexpr int A = HD / 64, B = (HD / 32) & 1, C = (HD / 16) & 1;
 #pragma unroll
     for (int i = 0; i < A; ++i) {
-        const uint4 v = *reinterpret_cast<const uint4*>(row + i * 128 + n * 16);
+        const uint4 v = lds<uint4>(rows + (HD % 128 == 0 ? (at ^ ((i & 1) * 64)) + (i >> 1) * 128 : at + i * 64));
         w[4 * i] = v.x; w[4 * i + 1] = v.y; w[4 * i + 2] = v.z; w[4 * i + 3] = v.w;
     }
     if (B) {
-        const uint2 v = *reinterpret_cast<const uint2*>(row + 128 * A + n * 8);
+        const uint2 v = lds<uint2>(rows + n * HD + 64 * A + c * 8);
         w[4 * A] = v.x; w[4 * A + B] = v.y;
     }
-    if (C) w[4 * A + 2 * B] = *reinterpret_cast<const uint32_t*>(row + 128 * A + 64 * B + n * 4);
-    if (D) w[VW - 1] = *reinterpret_cast<const uint16_t*>(row + 128 * A + 64 * B + 32 * C + n * 2);
+    if (C) w[KS - 1] = lds<uint32_t>(rows + n * HD + 64 * A + 32 * B + c * 4);
 }
+// Row 2 c + e of eight; at = where row 2 c's first bytes of this lane lie.
+__device__ __forceinline__ uint32_t value_at(int n, int c) {
+    if constexpr (HD == 64) return value_chunk(2 * c, n >> 1) + (n & 1) * 8;
+    else if constexpr (HD >= 128) return value_chunk(2 * c, n);
+    else return 2 * c * HD + (HD >= 64 ? n * 8 : 0);
+}
+__device__ __forceinline__ void load_value(uint32_t (&w)[VW], uint32_t rows, uint32_t at, int n, int c, int e) {
+    constexpr int A = HD / 128, B = (HD / 64) & 1, C = (HD / 32) & 1, D = (HD / 16) & 1;
+#pragma unroll
+    for (int i = 0; i < A; ++i) {
+        const uint4 v = lds<uint4>(rows + at + e * HD + i * 128);
+        w[4 * i] = v.x; w[4 * i + 1] = v.y; w[4 * i + 2] = v.z; w[4 * i + 3] = v.w;
+    }
+    const uint32_t row = rows + (2 * c + e) * HD + 128 * A;
+    if (B) {
+        const uint2 v = lds<uint2>(HD == 64 ? rows + (at ^ (e * 64)) : HD < 128 ? rows + at + e * HD : row + n * 8);
+        w[4 * A] = v.x; w[4 * A + B] = v.y;
+    }
+    if (C) w[4 * A + 2 * B] = lds<uint32_t>(row + 64 * B + n * 4);
+    if (D) {                                         // two bytes; the load takes the four that they lie in
+        const uint32_t v = lds<uint32_t>(row + 64 * B + 32 * C + (n & ~1) * 2);
+        w[VW - 1] = n & 1 ? v >> 16 : v & 0xffffu;
+    }
+}
+__device__ __forceinline__ void cp_async16(uint32_t dst, const void* src) {
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
+}
+__device__ __forceinline__ void cp_async4(uint32_t dst, const void* src) {
+    asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(dst), "l"(src) : "memory");
+}
+__device__ __forceinline__ void cp_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N> __device__ __forceinline__ void cp_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
 
 struct Cache {
     const uint8_t *k, *v;
@@ -142,280 +188,357 @@ struct Walk {
 
 // -------------------------------------------------------------------------------------------- few rows
 constexpr int MAX_CLUSTER = 8;
-constexpr size_t stream_smem(int ng) {           // queries' fragments; then the warps' results, what a CTA shows to its cluster
-    return (size_t)ng * KS * 32 * 8 + (size_t)(WARPS + 1) * 8 * ng * (HD + 2) * 4;
-}
+constexpr int MAX_CTAS = 6 * PLM_SM_COUNT;       // (a float a warp fits the second kernel's shared memory)
+constexpr int ROW = HD + 2;                      // floats of a partial result's row: sums, maximum, denominator
+template <int NG> struct Few {
+    enum : int {
+        SB = HD * NG <= 256 && HD <= 128 ? 2 : 1,                    // blocks of 16 keys at a time
+        KB = 16 * SB,
+        TILE = KB * HD,                                              // bytes of KB keys
+        STAGES = TILE >= 4096 ? 2 : TILE >= 2048 ? 3 : 4,            // units a warp has in its ring
+        CTAS = NG == 1 ? (HD <= 64 ? 4 : HD <= 128 ? 3 : 2) : NG == 2 && HD <= 64 ? 3 : 2,      // an SM
+        Q_BYTES = NG > 1 ? WARPS * NG * KS * 32 * 8 : 0,             // the queries' fragments (of one group: in registers)
+        RING = WARPS * STAGES * 2 * TILE,
+        AFTER = (WARPS + 1) * 8 * NG * ROW * 4,                      // the warps' results, what a CTA shows to its cluster
+        SMEM = Q_BYTES + (RING > AFTER ? (int)RING : (int)AFTER),
+    };
+};
 
-// grid (ranges, G * tiles, sequences); NG groups of 8 (token, head) rows a CTA.  See Kv8Step for what a sequence is.
+// The rows of one sequence and kv head, COLS at a time, against its keys: how the work is dealt out.  A sequence's walk is one of
+// units of KB keys, the same for all its tiles of rows and kv heads; all walks of the step in a row (sequence by sequence, and
+// there (kv head, tile) by (kv head, tile)) are cut into one equal range for each warp.  So a ragged batch keeps all SMs busy to the
+// end; a warp meets at most two walks that are not wholly its own, and leaves partial results for those.
+constexpr int MIN_UNITS = 4;                     // of a warp's range, so that its start and a partial result are worth it
+template <int COLS, int KB> struct Deal {
+    const Kv8Step& step;
+    int n_seqs, G, R, window, keep;
+    __device__ __forceinline__ void of(int b, int& units, int& tiles) const {
+        const Kv8Seq q = kv8_seq(step, b);
+        units = tiles = 0;
+        if (q.n_new <= 0) return;
+        const int last = q.pos0 + q.n_new - 1;
+        const Walk w(q.pos0, last, window, keep);
+        units = w.n_pages * (PLM_PAGE / KB) - (PLM_PAGE - 1 - last % PLM_PAGE) / KB;
+        tiles = (q.n_new * R + COLS - 1) / COLS;
+    }
+    __device__ __forceinline__ unsigned long long all(int b) const {
+        int u, t;
+        of(b, u, t);
+        return (unsigned long long)u * t * G;
+    }
+    // A whole warp, number `w` of n_warps: its units of all, and the sequence that the first belongs to with the units before that.
+    __device__ __forceinline__ bool range(int w, int n_warps, unsigned long long& per, unsigned long long& at, unsigned long long& end, int& b,
+                                          unsigned long long& before) const {
+        constexpr int HOLD = 4;                                      // 128 sequences are asked for once
+        const int lane = threadIdx.x & 31;
+        unsigned long long held[HOLD], total = 0;
+#pragma unroll
+        for (int i = 0; i < HOLD; ++i) total += held[i] = i * 32 + lane < n_seqs ? all(i * 32 + lane) : 0;
+        for (int i = HOLD * 32 + lane; i < n_seqs; i += 32) total += all(i);
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1) total += __shfl_xor_sync(0xffffffffu, total, o);
+        per = (total + n_warps - 1) / n_warps;
+        per = per < MIN_UNITS ? MIN_UNITS : per;
+        at = per * w;
+        end = at + per < total ? at + per : total;
+        if (at >= end) return false;
+        before = 0;
+        for (int i0 = 0; i0 < n_seqs; i0 += 32) {
+            const unsigned long long mine = i0 == 0 ? held[0] : i0 == 32 ? held[1] : i0 == 64 ? held[2] : i0 == 96 ? held[3]
+                                                                                                          : i0 + lane < n_seqs ? all(i0 + lane) : 0;
+            unsigned long long sum = mine;
+#pragma unroll
+            for (int o = 1; o < 32; o <<= 1) {
+                const unsigned long long x = __shfl_up_sync(0xffffffffu, sum, o);
+                if (lane >= o) sum += x;
+            }
+            const unsigned here = __ballot_sync(0xffffffffu, before + sum > at);
+            if (here) {
+                const int f = __ffs(here) - 1;
+                before += __shfl_sync(0xffffffffu, sum - mine, f);
+                b = i0 + f;
+                return true;
+            }
+            before += __shfl_sync(0xffffffffu, sum, 31);
+        }
+        return false;
+    }
+};
+
+// NG groups of 8 (token, head) rows a warp.  CLUSTER: grid (ranges, G * tiles, sequences), the ranges of a walk are the CTAs of a
+// cluster.  Else: any number of warps, see Deal; `ws` holds two partial results a warp: [0] of a walk that an earlier warp began,
+// [1] of one that a later warp ends, each [COLS][ROW], and `pieces` [n_seqs * G * tiles] which warp began each walk and how many
+// have a piece of it.
 template <int NG, bool CLUSTER>
-__global__ void __launch_bounds__(NT)
-kv8_stream_kernel(const bf16* q, const Cache cache, bf16* __restrict__ out, float* __restrict__ ws, const Kv8Step step, int H, int G,
-                  int tiles, float scale_log2, int window, const float* sink, int keep, const float* slopes) {
-    constexpr int COLS = 8 * NG;
-    extern __shared__ __align__(16) uint8_t sm_raw[];
-    uint2* q_frag = reinterpret_cast<uint2*>(sm_raw);                              // [NG][KS][32]
-    float* part = reinterpret_cast<float*>(sm_raw + (size_t)NG * KS * 32 * 8);     // [WARPS][COLS][HD + 2]
-    float* mine = part + WARPS * COLS * (HD + 2);                                  // [COLS][HD + 2]
-    __shared__ int row_exp[COLS];
-    __shared__ int s_nan;                        // a value that not all rows see is NaN: looked at again at the end
+__global__ void __launch_bounds__(NT, Few<NG>::CTAS)
+kv8_stream_kernel(const bf16* q, const Cache cache, bf16* __restrict__ out, float* __restrict__ ws, int2* __restrict__ pieces, const Kv8Step step,
+                  int n_seqs, int H, int G, int tiles, float scale_log2, int window, const float* sink, int keep, const float* slopes) {
+    constexpr int COLS = 8 * NG, SB = Few<NG>::SB, KB = Few<NG>::KB, TILE = Few<NG>::TILE, STAGES = Few<NG>::STAGES;
+    constexpr unsigned UNITS = PLM_PAGE / KB;
+    extern __shared__ __align__(128) uint8_t sm_raw[];                             // [WARPS][NG][KS][32] queries, [WARPS][STAGES][keys, values]
+    __shared__ float scales[WARPS][STAGES][2];
     pdl_wait();
     pdl_launch_dependents();
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, n8 = lane >> 2, c4 = lane & 3;
-    const int g = blockIdx.y / tiles, tile = blockIdx.y - g * tiles, R = H / G;
-    const int n_splits = gridDim.x, split = blockIdx.x;
-    const Kv8Seq sq = kv8_seq(step, blockIdx.z);
-    const int pair0 = tile * COLS, n_pairs = sq.n_new * R;
-    if (pair0 >= n_pairs) return;                                                  // (with all CTAs of its cluster)
-    const int n_cols = min(COLS, n_pairs - pair0);
-    const int pos_first = sq.pos0 + pair0 / R, pos_last = sq.pos0 + (pair0 + n_cols - 1) / R;
-    const int lo_first = plm_first_key(pos_first, window), lo_last = plm_first_key(pos_last, window);
-    if (threadIdx.x == 0) s_nan = 0;
+    const int R = H / G;
+    uint2* q_frag = reinterpret_cast<uint2*>(sm_raw) + (NG > 1 ? warp * NG * KS * 32 : 0);
+    const uint32_t ring = smem_u32(sm_raw + Few<NG>::Q_BYTES) + warp * STAGES * 2 * TILE, scales_s = smem_u32(&scales[warp][0][0]);
+    const uint32_t key_to = key_chunk(lane / (HD / 16), lane % (HD / 16)), value_to = value_chunk(lane / (HD / 16), lane % (HD / 16));
+    const uint32_t key_from = key_chunk(n8, c4), value_from = value_at(n8, c4);
 
-    // the queries as B operands: warp by warp a group of 8 rows, row n8's components key_component(w, c4) .. + 3
-    for (int ng = warp; ng < NG; ng += WARPS) {
-        const int pair = pair0 + ng * 8 + n8;
-        const bool have = pair < n_pairs;
-        const bf16* row = q + ((size_t)(sq.t0 + (have ? pair / R : 0)) * H + g * R + (have ? pair % R : 0)) * HD;
-        uint2 w[KS];
-        float most = 0.f;
-#pragma unroll
-        for (int s = 0; s < KS; ++s) {
-            w[s] = have ? *reinterpret_cast<const uint2*>(row + key_component(s, c4)) : make_uint2(0, 0);
-            most = fmaxf(fmaxf(fmaxf(kv8_magnitude(__uint_as_float(w[s].x << 16)), kv8_magnitude(__uint_as_float(w[s].x & 0xffff0000u))),
-                               fmaxf(kv8_magnitude(__uint_as_float(w[s].y << 16)), kv8_magnitude(__uint_as_float(w[s].y & 0xffff0000u)))), most);
-        }
-        most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, 1));
-        most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, 2));
-        const int e = row_exponent(most);
-        const float down = kv8_pow2(-e);
-#pragma unroll
-        for (int s = 0; s < KS; ++s)
-            q_frag[(ng * KS + s) * 32 + lane] =
-                make_uint2(halves(__uint_as_float(w[s].x << 16) * down, __uint_as_float(w[s].x & 0xffff0000u) * down),
-                           halves(__uint_as_float(w[s].y << 16) * down, __uint_as_float(w[s].y & 0xffff0000u) * down));
-        if (c4 == 0) row_exp[ng * 8 + n8] = e;
-    }
+    // A warp's piece: units u0, u0 + stride, .. below u1 of the walk of rows pair0 .. of sequence sq and kv head g.  finish(o, m, l): the sums
+    // out^T in units of 1, maximum and denominator of this lane's rows 8 j + 2 c4 and + 1.
+    auto piece = [&](const Kv8Seq& sq, int g, int tile, int u0, int u1, int stride, auto&& finish) {
+        const int pair0 = tile * COLS, n_pairs = sq.n_new * R;
+        const int n_cols = min(COLS, n_pairs - pair0);
+        const int pos_first = sq.pos0 + pair0 / R, pos_last = sq.pos0 + (pair0 + n_cols - 1) / R;
+        const int lo_first = plm_first_key(pos_first, window), lo_last = plm_first_key(pos_last, window);
+        const Walk walk(sq.pos0, sq.pos0 + sq.n_new - 1, window, keep);
 
-    // the warp's range of units of KB keys
-    const Walk walk(pos_first, pos_last, window, keep);
-    const int n_units = walk.n_pages * UNITS, per = (n_units + n_splits * WARPS - 1) / (n_splits * WARPS);
-    const int u0 = (split * WARPS + warp) * per, u1 = min(n_units, u0 + per);
-    auto number = [&](int u) { return PLM_PAGE_NO(sq.pages[walk.page_at(u / UNITS)]); };
-    uint32_t kw[SB][2][KS], vw[SB][4][VW];
-    float ks = 0.f, vs = 1.f;
-    auto load_keys = [&](int u, int page) {
-        const uint8_t* at = cache.k + (((size_t)page * G + g) * PLM_PAGE + u % UNITS * KB + n8) * HD;
+        // The ring's first units are asked for before the queries are looked at.  A unit's keys and values are groups of their own, each
+        // asked for as soon as its place is free.
+        auto number = [&](unsigned u) { return PLM_PAGE_NO(sq.pages[walk.page_at((int)(u / UNITS))]); };
+        auto offset = [&](unsigned u, unsigned block) { return (size_t)block * (PLM_PAGE * HD) + u % UNITS * TILE; };
+        constexpr int CHUNKS = TILE / 16;
+        auto ask_keys = [&](unsigned u, unsigned block, int stage) {
+            const uint8_t* from = cache.k + offset(u, block) + lane * 16;
+            const uint32_t to = ring + stage * (2 * TILE);
 #pragma unroll
-        for (int b = 0; b < SB; ++b) {
-            load_key(kw[b][0], at + b * 16 * HD, c4);
-            load_key(kw[b][1], at + (b * 16 + 8) * HD, c4);
-        }
-    };
-    auto load_values = [&](int u, int page) {                        // keys 2 c4, 2 c4 + 1, and those plus 8
-        const uint8_t* at = cache.v + (((size_t)page * G + g) * PLM_PAGE + u % UNITS * KB + 2 * c4) * HD;
+            for (int x = 0; x < CHUNKS; x += 32)
+                if (CHUNKS % 32 == 0 || x + lane < CHUNKS) cp_async16(to + key_place(key_to, x / 32), from + x * 16);
+            if (lane < 2) cp_async4(scales_s + (stage * 2 + lane) * 4, (lane ? cache.vs : cache.ks) + block);
+        };
+        auto ask_values = [&](unsigned u, unsigned block, int stage) {
+            const uint8_t* from = cache.v + offset(u, block) + lane * 16;
+            const uint32_t to = ring + stage * (2 * TILE) + TILE;
 #pragma unroll
-        for (int b = 0; b < SB; ++b)
+            for (int x = 0; x < CHUNKS; x += 32)
+                if (CHUNKS % 32 == 0 || x + lane < CHUNKS) cp_async16(to + value_place(value_to, x / 32), from + x * 16);
+        };
+        unsigned block = 0;                                          // page and kv head of the unit asked for last
+        int page_next = 0;                                           // page of the one after it
 #pragma unroll
-            for (int i = 0; i < 4; ++i) load_value(vw[b][i], at + (b * 16 + (i & 1) + (i >> 1) * 8) * HD, n8);
-    };
-    int page = 0, page_next = 0;
-    if (u0 < u1) {
-        page = number(u0);
-        ks = cache.ks[(size_t)page * G + g];
-        vs = cache.vs[(size_t)page * G + g];
-        load_keys(u0, page);
-        load_values(u0, page);
-        page_next = number(min(u0 + 1, u1 - 1));
-    }
-    __syncthreads();                                                 // the queries' fragments are there
-
-    // this lane's columns of S^T and out^T: rows 8 j + 2 c4 and + 1
-    float m[NG][2], l[NG][2], cs[NG][2], slope[NG][2];
-    int pos[NG][2], lo[NG][2];
-#pragma unroll
-    for (int j = 0; j < NG; ++j)
-#pragma unroll
-        for (int e = 0; e < 2; ++e) {
-            const int pair = pair0 + j * 8 + c4 * 2 + e;
-            const bool have = pair < n_pairs;
-            m[j][e] = -INFINITY;
-            l[j][e] = 0.f;
-            cs[j][e] = have ? scale_log2 * kv8_pow2(max(-126, min(127, row_exp[j * 8 + c4 * 2 + e]))) : 0.f;
-            slope[j][e] = slopes && have ? slopes[g * R + pair % R] * LOG2E : 0.f;
-            pos[j][e] = have ? sq.pos0 + pair / R : -1;
-            lo[j][e] = plm_first_key(pos[j][e], window);
-        }
-    float o[NG][MT][4];
-#pragma unroll
-    for (int j = 0; j < NG; ++j)
-#pragma unroll
-        for (int t = 0; t < MT; ++t) o[j][t][0] = o[j][t][1] = o[j][t][2] = o[j][t][3] = 0.f;
-    uint2 qr[NG == 1 ? KS : 1];
-    if (NG == 1) {
-#pragma unroll
-        for (int s = 0; s < KS; ++s) qr[NG == 1 ? s : 0] = q_frag[s * 32 + lane];
-    }
-    int eo = kv8_exponent_of_scale(vs);
-
-    for (int u = u0; u < u1; ++u) {
-        const int key0 = walk.page_at(u / UNITS) * PLM_PAGE + u % UNITS * KB;
-        const bool edge = key0 + KB - 1 > pos_first || key0 < lo_last;
-        float s[SB][NG][4];
-#pragma unroll
-        for (int b = 0; b < SB; ++b)
-#pragma unroll
-            for (int j = 0; j < NG; ++j) s[b][j][0] = s[b][j][1] = s[b][j][2] = s[b][j][3] = 0.f;
-#pragma unroll
-        for (int w = 0; w < KS; ++w) {
-            uint32_t a[SB][4];
-#pragma unroll
-            for (int b = 0; b < SB; ++b) {
-                a[b][0] = kv8_halves(kw[b][0][w] & 0xffffu);
-                a[b][1] = kv8_halves(kw[b][1][w] & 0xffffu);
-                a[b][2] = kv8_halves(kw[b][0][w] >> 16);
-                a[b][3] = kv8_halves(kw[b][1][w] >> 16);
-            }
-#pragma unroll
-            for (int j = 0; j < NG; ++j) {
-                const uint2 f = NG == 1 ? qr[NG == 1 ? w : 0] : q_frag[(j * KS + w) * 32 + lane];
-#pragma unroll
-                for (int b = 0; b < SB; ++b) mma_f16(s[b][j], a[b], f.x, f.y);
+        for (int i = 0; i < STAGES; ++i) {
+            if (u0 + i * stride < u1) {
+                block = (unsigned)number(u0 + i * stride) * G + g;
+                ask_keys(u0 + i * stride, block, i);
+                cp_commit();
+                ask_values(u0 + i * stride, block, i);
+                cp_commit();
+            } else {
+                cp_commit();
+                cp_commit();
             }
         }
-        // the next unit's keys into the registers that are free now, its page's number having come with the last
-        const float ks_now = ks, vs_now = vs;
-        page = page_next;
-        if (u + 1 < u1) {
-            ks = cache.ks[(size_t)page * G + g];
-            vs = cache.vs[(size_t)page * G + g];
-            load_keys(u + 1, page);
-            page_next = number(min(u + 2, u1 - 1));
-        }
-        float mx[NG][2];
+        if (u0 + STAGES * stride < u1) page_next = number(u0 + STAGES * stride);
+
+        // The queries as B operands, a group of 8 rows at a time: this lane has row n8's components key_component(w, c4) .. + 3.
+        float m[NG][2], l[NG][2], cs[NG][2];
+        uint2 qr[NG == 1 ? KS : 1];
 #pragma unroll
         for (int j = 0; j < NG; ++j) {
+            const int pair = pair0 + j * 8 + n8;
+            const bool have = pair < n_pairs;
+            const bf16* row = q + ((size_t)(sq.t0 + (have ? pair / R : 0)) * H + g * R + (have ? pair % R : 0)) * HD;
+            uint2 w[KS];
+            float most = 0.f;
 #pragma unroll
-            for (int e = 0; e < 2; ++e) {
-                const float c = cs[j][e] * ks_now;
-                mx[j][e] = -INFINITY;
+            for (int s = 0; s < KS; ++s) w[s] = have ? *reinterpret_cast<const uint2*>(row + key_component(s, c4)) : make_uint2(0, 0);
 #pragma unroll
-                for (int b = 0; b < SB; ++b)
+            for (int s = 0; s < KS; ++s)
+                most = fmaxf(fmaxf(fmaxf(kv8_magnitude(__uint_as_float(w[s].x << 16)), kv8_magnitude(__uint_as_float(w[s].x & 0xffff0000u))),
+                                   fmaxf(kv8_magnitude(__uint_as_float(w[s].y << 16)), kv8_magnitude(__uint_as_float(w[s].y & 0xffff0000u)))), most);
+            most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, 1));
+            most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, 2));
+            const int e = row_exponent(most);
+            const float down = kv8_pow2(-e);
 #pragma unroll
-                    for (int hi = 0; hi < 2; ++hi) s[b][j][2 * hi + e] *= c;
+            for (int s = 0; s < KS; ++s) {
+                const uint2 f = make_uint2(halves(__uint_as_float(w[s].x << 16) * down, __uint_as_float(w[s].x & 0xffff0000u) * down),
+                                           halves(__uint_as_float(w[s].y << 16) * down, __uint_as_float(w[s].y & 0xffff0000u) * down));
+                if (NG == 1) qr[NG == 1 ? s : 0] = f;
+                else q_frag[(j * KS + s) * 32 + lane] = f;           // (its reader is this lane)
             }
-            if (slopes) {
 #pragma unroll
-                for (int b = 0; b < SB; ++b)
-#pragma unroll
-                    for (int i = 0; i < 4; ++i)
-                        s[b][j][i] = fmaf(slope[j][i & 1], (float)(key0 + b * 16 + n8 + (i >> 1) * 8 - pos[j][i & 1]), s[b][j][i]);
+            for (int k = 0; k < 2; ++k) {
+                m[j][k] = -INFINITY;
+                l[j][k] = 0.f;
+                cs[j][k] = scale_log2 * kv8_pow2(max(-126, min(127, __shfl_sync(0xffffffffu, e, (c4 * 2 + k) * 4))));
             }
+        }
+        float o[NG][MT][4];
+#pragma unroll
+        for (int j = 0; j < NG; ++j)
+#pragma unroll
+            for (int t = 0; t < MT; ++t) o[j][t][0] = o[j][t][1] = o[j][t][2] = o[j][t][3] = 0.f;
+        int eo = 0, stage = 0;
+        bool nan_found = false;
+        for (int u = u0; u < u1; u += stride) {
+            const uint32_t tile = ring + stage * (2 * TILE);
+            const int key0 = walk.page_at((int)((unsigned)u / UNITS)) * PLM_PAGE + (int)((unsigned)u % UNITS) * KB;
+            const bool edge = key0 + KB - 1 > pos_first || key0 < lo_last;
+            float s[SB][NG][4];
+#pragma unroll
+            for (int b = 0; b < SB; ++b)
+#pragma unroll
+                for (int j = 0; j < NG; ++j) s[b][j][0] = s[b][j][1] = s[b][j][2] = s[b][j][3] = 0.f;
+            cp_wait<2 * STAGES - 1>();                               // this unit's keys are there
+            __syncwarp();
+            const float ks_now = scales[warp][stage][0];
+            const int ev = kv8_exponent_of_scale(scales[warp][stage][1]);
+            uint32_t kw[SB][2][KS];
+#pragma unroll
+            for (int b = 0; b < SB; ++b) {
+                load_key(kw[b][0], tile + b * 16 * HD, key_from, n8, c4);
+                load_key(kw[b][1], tile + (b * 16 + 8) * HD, key_from, n8, c4);
+            }
+#pragma unroll
+            for (int w = 0; w < KS; ++w) {
+                uint32_t a[SB][4];
+#pragma unroll
+                for (int b = 0; b < SB; ++b) {
+                    kv8_halves(kw[b][0][w], a[b][0], a[b][2]);
+                    kv8_halves(kw[b][1][w], a[b][1], a[b][3]);
+                }
+#pragma unroll
+                for (int j = 0; j < NG; ++j) {
+                    const uint2 f = NG == 1 ? qr[NG == 1 ? w : 0] : q_frag[(j * KS + w) * 32 + lane];
+#pragma unroll
+                    for (int b = 0; b < SB; ++b) mma_f16(s[b][j], a[b], f.x, f.y);
+                }
+            }
+            __syncwarp();                                            // its place is free
+            const bool more = u + STAGES * stride < u1;
+            if (more) {
+                block = (unsigned)page_next * G + g;
+                ask_keys(u + STAGES * stride, block, stage);
+                page_next = number(min(u + (STAGES + 1) * stride, u1 - 1));
+            }
+            cp_commit();
+            // scores in log2 units are s * c (with slopes and masks they are made here, and c is 1)
+            float c[NG][2], mx[NG][2];
+#pragma unroll
+            for (int j = 0; j < NG; ++j)
+#pragma unroll
+                for (int e = 0; e < 2; ++e) c[j][e] = cs[j][e] * ks_now;
+            if (edge || slopes) {
+#pragma unroll
+                for (int j = 0; j < NG; ++j)
+#pragma unroll
+                    for (int e = 0; e < 2; ++e) {
+                        const int pair = pair0 + j * 8 + c4 * 2 + e;
+                        const int pos = pair < n_pairs ? sq.pos0 + pair / R : -1, lo = plm_first_key(pos, window);
+                        const float slope = slopes && pair < n_pairs ? slopes[g * R + pair % R] * LOG2E : 0.f;
+#pragma unroll
+                        for (int b = 0; b < SB; ++b)
+#pragma unroll
+                            for (int hi = 0; hi < 2; ++hi) {
+                                const int key = key0 + b * 16 + n8 + hi * 8;
+                                const float x = fmaf(slope, (float)(key - pos), s[b][j][2 * hi + e] * c[j][e]);
+                                s[b][j][2 * hi + e] = key > pos || (key < lo && key >= keep) ? -INFINITY : x;
+                            }
+                        c[j][e] = 1.f;
+                    }
+            }
+            bool raise = false;
+#pragma unroll
+            for (int j = 0; j < NG; ++j)
+#pragma unroll
+                for (int e = 0; e < 2; ++e) {
+                    float x = fmaxf(s[0][j][e], s[0][j][2 + e]);
+                    if (SB == 2) x = fmaxf(x, fmaxf(s[SB - 1][j][e], s[SB - 1][j][2 + e]));
+                    x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 4));
+                    x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 8));
+                    x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 16));
+                    mx[j][e] = x * c[j][e];                          // (c is positive)
+                    raise |= mx[j][e] > (m[j][e] == -INFINITY ? -INFINITY : m[j][e] + RAISE);
+                }
+            int d = ev - eo;
+            if (__any_sync(0xffffffffu, raise || d > UNIT_SPAN || d < -UNIT_SPAN)) {
+#pragma unroll
+                for (int j = 0; j < NG; ++j) {
+                    float down[2];
+#pragma unroll
+                    for (int e = 0; e < 2; ++e) {
+                        const bool up = mx[j][e] > m[j][e];
+                        const float by = up ? m[j][e] - mx[j][e] : 0.f;            // -inf where nothing was seen before
+                        down[e] = ex2(by - (float)d);
+                        l[j][e] *= ex2(by);
+                        if (up) m[j][e] = mx[j][e];
+                    }
+#pragma unroll
+                    for (int t = 0; t < MT; ++t) {
+                        o[j][t][0] *= down[0]; o[j][t][1] *= down[1];
+                        o[j][t][2] *= down[0]; o[j][t][3] *= down[1];
+                    }
+                }
+                eo = ev;
+                d = 0;
+            }
+            uint32_t pf[SB][NG][2];
+            const float back = kv8_pow2(-d);
+#pragma unroll
+            for (int j = 0; j < NG; ++j) {
+                float sum[2] = {0.f, 0.f}, off[2];
+#pragma unroll
+                for (int e = 0; e < 2; ++e) off[e] = (float)d - (m[j][e] == -INFINITY ? 0.f : m[j][e]);
+#pragma unroll
+                for (int b = 0; b < SB; ++b) {
+                    float p[4];
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        p[i] = ex2(fmaf(s[b][j][i], c[j][i & 1], off[i & 1]));
+                        sum[i & 1] += p[i];
+                    }
+                    pf[b][j][0] = turned(halves(p[0], p[1]));
+                    pf[b][j][1] = turned(halves(p[2], p[3]));
+                }
+#pragma unroll
+                for (int e = 0; e < 2; ++e) l[j][e] = fmaf(sum[e], back, l[j][e]);
+            }
+            cp_wait<2 * STAGES - 1>();                               // its values are there
+            __syncwarp();
+            uint32_t vw[SB][4][VW];
+#pragma unroll
+            for (int b = 0; b < SB; ++b)
+#pragma unroll
+                for (int k = 0; k < 4; ++k) load_value(vw[b][k], tile + TILE + (b * 16 + (k >> 1) * 8) * HD, value_from, n8, c4, k & 1);
             if (edge) {
+                // Places that no row sees hold whatever was left there: zeros.  A NaN that some rows see and others do not would
+                // reach them all (0 * NaN): it is taken out, and put into the results of those that see it at the end.
 #pragma unroll
                 for (int b = 0; b < SB; ++b)
 #pragma unroll
                     for (int i = 0; i < 4; ++i) {
-                        const int key = key0 + b * 16 + n8 + (i >> 1) * 8;
-                        if (key > pos[j][i & 1] || (key < lo[j][i & 1] && key >= keep)) s[b][j][i] = -INFINITY;
+                        const int key = key0 + b * 16 + 2 * c4 + (i & 1) + (i >> 1) * 8;
+                        const bool seen = key <= pos_last && (key >= lo_first || key < keep);
+#pragma unroll
+                        for (int w = 0; w < VW; ++w) {
+                            const uint32_t marks = nan_bytes(vw[b][i][w]);
+                            nan_found |= seen && marks;
+                            vw[b][i][w] = seen ? without(vw[b][i][w], marks) : 0u;
+                        }
                     }
             }
 #pragma unroll
             for (int b = 0; b < SB; ++b)
-#pragma unroll
-                for (int i = 0; i < 4; ++i) mx[j][i & 1] = fmaxf(mx[j][i & 1], s[b][j][i]);
-        }
-        bool raise = false;
-#pragma unroll
-        for (int j = 0; j < NG; ++j)
-#pragma unroll
-            for (int e = 0; e < 2; ++e) {
-                mx[j][e] = fmaxf(mx[j][e], __shfl_xor_sync(0xffffffffu, mx[j][e], 4));
-                mx[j][e] = fmaxf(mx[j][e], __shfl_xor_sync(0xffffffffu, mx[j][e], 8));
-                mx[j][e] = fmaxf(mx[j][e], __shfl_xor_sync(0xffffffffu, mx[j][e], 16));
-                raise |= mx[j][e] > m[j][e] + RAISE || (m[j][e] == -INFINITY && mx[j][e] > -INFINITY);
-            }
-        const int ev = kv8_exponent_of_scale(vs_now);
-        int d = ev - eo;
-        if (__any_sync(0xffffffffu, raise) || d > UNIT_SPAN || d < -UNIT_SPAN) {
-#pragma unroll
-            for (int j = 0; j < NG; ++j) {
-                float down[2];
-#pragma unroll
-                for (int e = 0; e < 2; ++e) {
-                    const bool up = mx[j][e] > m[j][e];
-                    const float by = up ? m[j][e] - mx[j][e] : 0.f;                // -inf where nothing was seen before
-                    down[e] = ex2(by - (float)d);
-                    l[j][e] *= ex2(by);
-                    if (up) m[j][e] = mx[j][e];
-                }
 #pragma unroll
                 for (int t = 0; t < MT; ++t) {
-                    o[j][t][0] *= down[0]; o[j][t][1] *= down[1];
-                    o[j][t][2] *= down[0]; o[j][t][3] *= down[1];
+                    const uint32_t order = t & 1 ? 0x7362u : 0x5140u;
+                    const uint32_t x = __byte_perm(vw[b][0][t / 2], vw[b][1][t / 2], order);
+                    const uint32_t y = __byte_perm(vw[b][2][t / 2], vw[b][3][t / 2], order);
+                    uint32_t a[4];
+                    kv8_halves(x, a[0], a[1]);
+                    kv8_halves(y, a[2], a[3]);
+#pragma unroll
+                    for (int j = 0; j < NG; ++j) mma_f16(o[j][t], a, pf[b][j][0], pf[b][j][1]);
                 }
-            }
-            eo = ev;
-            d = 0;
+            __syncwarp();
+            if (more) ask_values(u + STAGES * stride, block, stage);
+            cp_commit();
+            stage = stage + 1 == STAGES ? 0 : stage + 1;
         }
-        uint32_t pf[SB][NG][2];
-        const float back = kv8_pow2(-d);
-#pragma unroll
-        for (int j = 0; j < NG; ++j) {
-            float sum[2] = {0.f, 0.f};
-            float off[2];
-#pragma unroll
-            for (int e = 0; e < 2; ++e) off[e] = (float)d - (m[j][e] == -INFINITY ? 0.f : m[j][e]);
-#pragma unroll
-            for (int b = 0; b < SB; ++b) {
-                float p[4];
-#pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    p[i] = ex2(s[b][j][i] + off[i & 1]);
-                    sum[i & 1] += p[i];
-                }
-                pf[b][j][0] = turned(halves(p[0], p[1]));
-                pf[b][j][1] = turned(halves(p[2], p[3]));
-            }
-#pragma unroll
-            for (int e = 0; e < 2; ++e) l[j][e] = fmaf(sum[e], back, l[j][e]);
-        }
-        if (edge) {
-            // Places that no row sees hold whatever was left there: zeros.  A NaN that some rows see and others do not would
-            // reach them all (0 * NaN): it is taken out, and put into the results of those that see it at the end.
-            bool found = false;
-#pragma unroll
-            for (int b = 0; b < SB; ++b)
-#pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    const int key = key0 + b * 16 + 2 * c4 + (i & 1) + (i >> 1) * 8;
-                    const bool seen = key <= pos_last && (key >= lo_first || key < keep);
-#pragma unroll
-                    for (int w = 0; w < VW; ++w) {
-                        const uint32_t marks = nan_bytes(vw[b][i][w]);
-                        found |= seen && marks;
-                        vw[b][i][w] = seen ? without(vw[b][i][w], marks) : 0u;
-                    }
-                }
-            if (found) s_nan = 1;
-        }
-#pragma unroll
-        for (int b = 0; b < SB; ++b)
-#pragma unroll
-            for (int t = 0; t < MT; ++t) {
-                const uint32_t order = t & 1 ? 0x7362u : 0x5140u;
-                const uint32_t x = __byte_perm(vw[b][0][t / 2], vw[b][1][t / 2], order);
-                const uint32_t y = __byte_perm(vw[b][2][t / 2], vw[b][3][t / 2], order);
-                const uint32_t a[4] = {kv8_halves(x & 0xffffu), kv8_halves(x >> 16), kv8_halves(y & 0xffffu), kv8_halves(y >> 16)};
-#pragma unroll
-                for (int j = 0; j < NG; ++j) mma_f16(o[j][t], a, pf[b][j][0], pf[b][j][1]);
-            }
-        if (u + 1 < u1) load_values(u + 1, page);
-    }
-
-    // the warps' results: part[warp][row] = sums in units of 1, [HD] = maximum, [HD + 1] = denominator
-    {
         const float unit = kv8_pow2(max(-126, min(127, eo)));
-        float* at = part + (size_t)warp * COLS * (HD + 2);
 #pragma unroll
         for (int j = 0; j < NG; ++j) {
 #pragma unroll
@@ -423,57 +546,83 @@ kv8_stream_kernel(const bf16* q, const Cache cache, bf16* __restrict__ out, floa
                 l[j][e] += __shfl_xor_sync(0xffffffffu, l[j][e], 4);
                 l[j][e] += __shfl_xor_sync(0xffffffffu, l[j][e], 8);
                 l[j][e] += __shfl_xor_sync(0xffffffffu, l[j][e], 16);
-                float* row = at + (j * 8 + c4 * 2 + e) * (HD + 2);
-#pragma unroll
-                for (int t = 0; t < MT; ++t)
-                    *reinterpret_cast<float2*>(row + value_component(t, n8)) = make_float2(o[j][t][e] * unit, o[j][t][2 + e] * unit);
-                if (n8 == 0) *reinterpret_cast<float2*>(row + HD) = make_float2(m[j][e], l[j][e]);
             }
-        }
-    }
-    __syncthreads();
-    for (int i = threadIdx.x; i < n_cols * HD; i += NT) {
-        const int col = i / HD, d = i - col * HD;
-        float mw[WARPS], mm = -INFINITY;
 #pragma unroll
-        for (int w = 0; w < WARPS; ++w) {
-            mw[w] = part[((size_t)w * COLS + col) * (HD + 2) + HD];
-            mm = fmaxf(mm, mw[w]);
-        }
-        float acc = 0.f, ll = 0.f;
+            for (int t = 0; t < MT; ++t)
 #pragma unroll
-        for (int w = 0; w < WARPS; ++w) {
-            const float wgt = mw[w] == -INFINITY ? 0.f : exp2f(mw[w] - mm);
-            acc = fmaf(wgt, part[((size_t)w * COLS + col) * (HD + 2) + d], acc);
-            ll = fmaf(wgt, part[((size_t)w * COLS + col) * (HD + 2) + HD + 1], ll);
+                for (int e = 0; e < 4; ++e) o[j][t][e] *= unit;
         }
-        const int pair = pair0 + col;
-        if (s_nan) {                                                 // the edge units of this CTA's range once more
-            const int p = sq.pos0 + pair / R, lo_p = plm_first_key(p, window);
-            const int end = min(n_units, (split + 1) * WARPS * per);
-            for (int u = split * WARPS * per; u < end; ++u) {
-                const int key0 = walk.page_at(u / UNITS) * PLM_PAGE + u % UNITS * KB;
+        if (__any_sync(0xffffffffu, nan_found)) {                    // the piece's edge units once more
+            for (int u = u0; u < u1; u += stride) {
+                const int key0 = walk.page_at((int)((unsigned)u / UNITS)) * PLM_PAGE + (int)((unsigned)u % UNITS) * KB;
                 if (!(key0 + KB - 1 > pos_first || key0 < lo_last)) continue;
-                const uint8_t* at = cache.v + (((size_t)number(u) * G + g) * PLM_PAGE + u % UNITS * KB) * HD + d;
+                const uint8_t* at = cache.v + offset(u, (unsigned)number(u) * G + g);
                 for (int k = 0; k < KB; ++k)
-                    if (key0 + k <= p && (key0 + k >= lo_p || key0 + k < keep) && is_nan_byte(at[(size_t)k * HD])) acc = __int_as_float(0x7fffffff);
+#pragma unroll
+                    for (int t = 0; t < MT; ++t) {
+                        const uint8_t* v = at + (size_t)k * HD + value_component(t, n8);
+                        const bool n0 = is_nan_byte(v[0]), n1 = is_nan_byte(v[1]);
+                        if (!(n0 || n1)) continue;
+#pragma unroll
+                        for (int j = 0; j < NG; ++j)
+#pragma unroll
+                            for (int e = 0; e < 2; ++e) {
+                                const int pair = pair0 + j * 8 + c4 * 2 + e, p = sq.pos0 + pair / R, lo = plm_first_key(p, window);
+                                if (pair >= n_pairs || key0 + k > p || (key0 + k < lo && key0 + k >= keep)) continue;
+                                if (n0) o[j][t][e] = __int_as_float(0x7fffffff);
+                                if (n1) o[j][t][2 + e] = __int_as_float(0x7fffffff);
+                            }
+                    }
             }
         }
-        const size_t row = (size_t)(sq.t0 + pair / R) * H + g * R + pair % R;
-        if (CLUSTER) {
-            mine[col * (HD + 2) + d] = acc;
-            if (d == 0) { mine[col * (HD + 2) + HD] = mm; mine[col * (HD + 2) + HD + 1] = ll; }
-        } else if (n_splits == 1) {
-            out[row * HD + d] = __float2bfloat16_rn(acc * kv8_inverse(mm, ll, sink ? sink + g * R + pair % R : nullptr));
-        } else {
-            float* at = ws + (row * n_splits + split) * (HD + 2);
-            at[d] = acc;
-            if (d == 0) { at[HD] = mm; at[HD + 1] = ll; }
+        finish(o, m, l);
+    };
+    // a lane's part of a row [ROW]: sums, maximum, denominator
+    auto put = [&](float* row, const float (&o)[MT][4], int e, float m, float l) {
+#pragma unroll
+        for (int t = 0; t < MT; ++t) *reinterpret_cast<float2*>(row + value_component(t, n8)) = make_float2(o[t][e], o[t][2 + e]);
+        if (n8 == 0) *reinterpret_cast<float2*>(row + HD) = make_float2(m, l);
+    };
+
+    const Deal<COLS, KB> deal = {step, n_seqs, G, R, window, keep};
+    if constexpr (CLUSTER) {
+        float* part = reinterpret_cast<float*>(sm_raw + Few<NG>::Q_BYTES);         // after the walk, in the rings' place: [WARPS][COLS][ROW]
+        float* mine = part + WARPS * COLS * ROW;                                   // [COLS][ROW]
+        const int g = blockIdx.y / tiles, tile = blockIdx.y - g * tiles, n_splits = gridDim.x, rank = blockIdx.x;
+        const Kv8Seq sq = kv8_seq(step, blockIdx.z);
+        int units, n_tiles;
+        deal.of(blockIdx.z, units, n_tiles);
+        if (tile >= n_tiles) return;                                               // (with all CTAs of its cluster)
+        const int per = (units + n_splits - 1) / n_splits;
+        const int pair0 = tile * COLS, n_cols = min(COLS, sq.n_new * R - pair0);
+        piece(sq, g, tile, min(units, rank * per) + warp, min(units, (rank + 1) * per), WARPS, [&](auto& o, auto& m, auto& l) {
+            __syncthreads();                                                       // all rings are free
+#pragma unroll
+            for (int j = 0; j < NG; ++j)
+#pragma unroll
+                for (int e = 0; e < 2; ++e)
+                    if (j * 8 + c4 * 2 + e < n_cols) put(part + (size_t)(warp * COLS + j * 8 + c4 * 2 + e) * ROW, o[j], e, m[j][e], l[j][e]);
+        });
+        __syncthreads();
+        for (int i = threadIdx.x; i < n_cols * HD; i += NT) {
+            const int col = i / HD, d = i - col * HD;
+            float mw[WARPS], mm = -INFINITY;
+#pragma unroll
+            for (int w = 0; w < WARPS; ++w) {
+                mw[w] = part[((size_t)w * COLS + col) * ROW + HD];
+                mm = fmaxf(mm, mw[w]);
+            }
+            float acc = 0.f, ll = 0.f;
+#pragma unroll
+            for (int w = 0; w < WARPS; ++w) {
+                const float wgt = mw[w] == -INFINITY ? 0.f : exp2f(mw[w] - mm);
+                acc = fmaf(wgt, part[((size_t)w * COLS + col) * ROW + d], acc);
+                ll = fmaf(wgt, part[((size_t)w * COLS + col) * ROW + HD + 1], ll);
+            }
+            mine[col * ROW + d] = acc;
+            if (d == 0) { mine[col * ROW + HD] = mm; mine[col * ROW + HD + 1] = ll; }
         }
-    }
-    if (CLUSTER) {
         cluster_sync_all();
-        const int rank = (int)cluster_rank();                        // == split
         for (int i = rank * NT + threadIdx.x; i < n_cols * HD; i += n_splits * NT) {
             const int col = i / HD, d = i - col * HD, pair = pair0 + col;
             float ms[MAX_CLUSTER], ls[MAX_CLUSTER], as[MAX_CLUSTER], mm = -INFINITY;
@@ -481,7 +630,7 @@ kv8_stream_kernel(const bf16* q, const Cache cache, bf16* __restrict__ out, floa
             for (int s = 0; s < MAX_CLUSTER; ++s) {
                 ms[s] = -INFINITY; ls[s] = 0.f; as[s] = 0.f;
                 if (s < n_splits) {
-                    const uint32_t at = cluster_map(mine + col * (HD + 2), (uint32_t)s);
+                    const uint32_t at = cluster_map(mine + col * ROW, (uint32_t)s);
                     ms[s] = cluster_ld_f32(at + HD * 4);
                     ls[s] = cluster_ld_f32(at + (HD + 1) * 4);
                     as[s] = cluster_ld_f32(at + d * 4);
@@ -496,49 +645,155 @@ kv8_stream_kernel(const bf16* q, const Cache cache, bf16* __restrict__ out, floa
                 acc = fmaf(wgt, as[s], acc);
                 ll = fmaf(wgt, ls[s], ll);
             }
-            out[((size_t)(sq.t0 + pair / R) * H + g * R + pair % R) * HD + d] =
-                __float2bfloat16_rn(acc * kv8_inverse(mm, ll, sink ? sink + g * R + pair % R : nullptr));
+            const int h = g * R + pair % R;
+            out[((size_t)(sq.t0 + pair / R) * H + h) * HD + d] = __float2bfloat16_rn(acc * kv8_inverse(mm, ll, sink ? sink + h : nullptr));
         }
         cluster_sync_all();                                          // nobody reads this CTA's shared memory any more
+    } else {
+        const int w = blockIdx.x * WARPS + warp;
+        unsigned long long per, at, end, before;
+        int b, units, n_tiles;
+        if (!deal.range(w, gridDim.x * WARPS, per, at, end, b, before)) return;
+        deal.of(b, units, n_tiles);
+        unsigned rest = (unsigned)((at - before) / units);           // (kv head, tile) within the sequence
+        int u0 = (int)(at - before - (unsigned long long)rest * units);
+        while (true) {
+            const int u1 = (int)min((unsigned long long)units, u0 + (end - at));
+            const int g = (int)rest / n_tiles, tile = (int)rest - g * n_tiles, pair0 = tile * COLS;
+            const Kv8Seq sq = kv8_seq(step, b);
+            const int n_cols = min(COLS, sq.n_new * R - pair0);
+            const bool whole = u0 == 0 && u1 == units;
+            float* where = ws + ((size_t)w * 2 + (u0 == 0 ? 1 : 0)) * COLS * ROW;
+            if (u0 == 0 && lane == 0)                                // this warp, and those whose range begins within the walk
+                pieces[((size_t)b * G + g) * tiles + tile] = make_int2(w, 1 + (int)((at + units - 1) / per - w));
+            piece(sq, g, tile, u0, u1, 1, [&](auto& o, auto& m, auto& l) {
+#pragma unroll
+                for (int j = 0; j < NG; ++j)
+#pragma unroll
+                    for (int e = 0; e < 2; ++e) {
+                        const int col = j * 8 + c4 * 2 + e, pair = pair0 + col;
+                        if (col >= n_cols) continue;
+                        if (whole) {
+                            const int h = g * R + pair % R;
+                            const float inv = kv8_inverse(m[j][e], l[j][e], sink ? sink + h : nullptr);
+                            bf16* row = out + ((size_t)(sq.t0 + pair / R) * H + h) * HD;
+#pragma unroll
+                            for (int t = 0; t < MT; ++t)
+                                *reinterpret_cast<__nv_bfloat162*>(row + value_component(t, n8)) = __floats2bfloat162_rn(o[j][t][e] * inv, o[j][t][2 + e] * inv);
+                        } else {
+                            put(where + col * ROW, o[j], e, m[j][e], l[j][e]);
+                        }
+                    }
+            });
+            at += u1 - u0;
+            if (at >= end) break;
+            __syncwarp();                                            // the ring and the queries' place are free
+            u0 = 0;
+            if (++rest == (unsigned)(n_tiles * G)) {
+                rest = 0;
+                do { deal.of(++b, units, n_tiles); } while (units == 0);
+            }
+        }
     }
 }
 
-// out[row] = sum_s w_s acc_s / sum_s w_s l_s with w_s = exp2(m_s - max m), ranges in their order.  A block a row.
-__global__ void __launch_bounds__(NT)
-kv8_join_kernel(const float* ws, bf16* __restrict__ out, int n_splits, int H, const float* sink, const int* seq_start, int n_seqs) {
-    extern __shared__ float weight[];                                // [n_splits]
-    __shared__ float red[NT / 32], s_l;
+// The partial results of walks that several warps shared: out[row] = sum_w f_w acc_w / sum_w f_w l_w with f_w = exp2(m_w - max m), warps in
+// their order.  A thread takes a component of a row, eight warps' results at a time, all asked for at once: two trips to memory for
+// most walks of a large step.  grid (G * tiles, 256ths of a tile's rows, sequences).
+constexpr int JOIN = 256, AT_ONCE = 8;
+template <int NG>
+__global__ void __launch_bounds__(JOIN)
+kv8_join_kernel(const float* ws, const int2* pieces, bf16* __restrict__ out, const Kv8Step step, int H, int G, int tiles, const float* sink) {
+    constexpr int COLS = 8 * NG;
     pdl_wait();
     pdl_launch_dependents();
-    const size_t row = blockIdx.x;
-    if (kv8_of_no_sequence((int)(row / H), seq_start, n_seqs)) return;
-    const float* p = ws + row * n_splits * (HD + 2);
+    const int R = H / G, b = blockIdx.z, at = blockIdx.y * JOIN + threadIdx.x, row = at / HD, d = at - row * HD;
+    const int g = blockIdx.x / tiles, tile = blockIdx.x - g * tiles, pair = tile * COLS + row;
+    const int t0 = step.tok_pos ? b : step.seq_start[b], n_new = step.tok_pos ? 1 : step.seq_start[b + 1] - t0;
+    if (tile * COLS >= n_new * R) return;                            // (no walk)
+    const int2 who = pieces[((size_t)b * G + g) * tiles + tile];
+    if (who.y == 1 || row >= COLS || pair >= n_new * R) return;      // one warp had it all, or no such row
+    auto place = [&](int i) { return ws + ((size_t)((who.x + i) * 2 + (i == 0 ? 1 : 0)) * COLS + row) * ROW; };
+    float m = -INFINITY, l = 0.f, acc = 0.f;
+    for (int i0 = 0; i0 < who.y; i0 += AT_ONCE) {
+        float ms[AT_ONCE], ls[AT_ONCE], as[AT_ONCE], top = m;
+#pragma unroll
+        for (int i = 0; i < AT_ONCE; ++i) {
+            const bool have = i0 + i < who.y;
+            const float* p = place(have ? i0 + i : i0);
+            ms[i] = p[HD]; ls[i] = p[HD + 1]; as[i] = p[d];
+            if (!have) ms[i] = -INFINITY;
+        }
+#pragma unroll
+        for (int i = 0; i < AT_ONCE; ++i) top = fmaxf(top, ms[i]);
+        if (top == -INFINITY) continue;
+        const float f = exp2f(m - top);
+        l *= f;
+        acc *= f;
+        m = top;
+#pragma unroll
+        for (int i = 0; i < AT_ONCE; ++i) {
+            if (ms[i] == -INFINITY) continue;
+            const float w = exp2f(ms[i] - top);
+            l = fmaf(w, ls[i], l);
+            acc = fmaf(w, as[i], acc);
+        }
+    }
+    const int h = g * R + pair % R;
+    out[((size_t)(t0 + pair / R) * H + h) * HD + d] = __float2bfloat16_rn(acc * kv8_inverse(m, l, sink ? sink + h : nullptr));
+}
+
+// The same for walks that many warps shared (few sequences): a block a row, in strands of every (512 / LANES)-th warp, the strands in
+// their order.  grid (G * tiles, rows of a tile, sequences).
+constexpr int LANES = HD <= 64 ? 64 : HD <= 128 ? 128 : 256;         // threads, one a component
+template <int NG>
+__global__ void __launch_bounds__(512)
+kv8_join_many_kernel(const float* ws, const int2* pieces, bf16* __restrict__ out, const Kv8Step step, int H, int G, int tiles, const float* sink) {
+    constexpr int COLS = 8 * NG, THREADS = 512, STRANDS = THREADS / LANES;
+    extern __shared__ float factor[];                                // one a warp of the walk
+    __shared__ float red[THREADS / 32], sums[THREADS];
+    pdl_wait();
+    pdl_launch_dependents();
+    const int R = H / G, b = blockIdx.z, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int g = blockIdx.x / tiles, tile = blockIdx.x - g * tiles, pair = tile * COLS + blockIdx.y;
+    const Kv8Seq sq = kv8_seq(step, b);
+    if (pair >= sq.n_new * R) return;
+    const int2 who = pieces[((size_t)b * G + g) * tiles + tile];
+    const int n = who.y;
+    if (n == 1) return;                                              // one warp had it all
+    auto place = [&](int i) { return ws + ((size_t)((who.x + i) * 2 + (i == 0 ? 1 : 0)) * COLS + blockIdx.y) * ROW; };
     float m = -INFINITY;
-    for (int s = threadIdx.x; s < n_splits; s += NT) m = fmaxf(m, p[(size_t)s * (HD + 2) + HD]);
+    for (int i = threadIdx.x; i < n; i += THREADS) m = fmaxf(m, factor[i] = place(i)[HD]);
     m = warp_max(m);
-    if ((threadIdx.x & 31) == 0) red[threadIdx.x >> 5] = m;
+    if (lane == 0) red[warp] = m;
     __syncthreads();
-    m = fmaxf(fmaxf(red[0], red[1]), fmaxf(red[2], red[3]));
-    for (int s = threadIdx.x; s < n_splits; s += NT) {
-        const float ms = p[(size_t)s * (HD + 2) + HD];
-        weight[s] = ms == -INFINITY ? 0.f : exp2f(ms - m);
+#pragma unroll
+    for (int k = 0; k < THREADS / 32; ++k) m = fmaxf(m, red[k]);
+    float l = 0.f;
+    for (int i = threadIdx.x; i < n; i += THREADS) {
+        const float f = factor[i] == -INFINITY ? 0.f : exp2f(factor[i] - m);
+        factor[i] = f;
+        l = fmaf(f, place(i)[HD + 1], l);
     }
+    l = warp_sum(l);
     __syncthreads();
-    if (threadIdx.x < 32) {                                          // ranges dealt out to 32 lanes, their sums in the tree's order
-        float l = 0.f;
-        for (int s = threadIdx.x; s < n_splits; s += 32)
-            if (weight[s] != 0.f) l = fmaf(weight[s], p[(size_t)s * (HD + 2) + HD + 1], l);
-        l = warp_sum(l);
-        if (threadIdx.x == 0) s_l = l;
-    }
-    __syncthreads();
-    const float inv = kv8_inverse(m, s_l, sink ? sink + row % H : nullptr);
-    for (int d = threadIdx.x; d < HD; d += NT) {
-        float acc = 0.f;
+    if (lane == 0) red[warp] = l;
+    const int strand = threadIdx.x / LANES, d = threadIdx.x % LANES;
+    float acc = 0.f;
+    if (d < HD) {
 #pragma unroll 8
-        for (int s = 0; s < n_splits; ++s)
-            if (weight[s] != 0.f) acc = fmaf(weight[s], p[(size_t)s * (HD + 2) + d], acc);
-        out[row * HD + d] = __float2bfloat16_rn(acc * inv);
+        for (int i = strand; i < n; i += STRANDS) acc = fmaf(factor[i], place(i)[d], acc);
+    }
+    sums[threadIdx.x] = acc;
+    __syncthreads();
+    if (strand == 0 && d < HD) {
+        l = 0.f;
+#pragma unroll
+        for (int k = 0; k < THREADS / 32; ++k) l += red[k];
+#pragma unroll
+        for (int k = 1; k < STRANDS; ++k) acc += sums[k * LANES + d];
+        const int h = g * R + pair % R;
+        out[((size_t)(sq.t0 + pair / R) * H + h) * HD + d] = __float2bfloat16_rn(acc * kv8_inverse(m, l, sink ? sink + h : nullptr));
     }
 }
 
@@ -553,7 +808,7 @@ kv8_tile_kernel(const bf16* q, const Cache cache, bf16* __restrict__ out, const 
                 const float* sink, int keep, const float* slopes) {
     constexpr int CPR = HD / 16, CHUNKS = 64 * CPR / NT > 0 ? (64 * CPR + NT - 1) / NT : 1;       // 16-byte chunks of a page's rows
     constexpr bool AHEAD = HD <= 128;
-    extern __shared__ __align__(16) uint8_t sm_raw[];
+    extern __shared__ __align__(128) uint8_t sm_raw[];
     __half* q_s = reinterpret_cast<__half*>(sm_raw);
     __half* k_s = q_s + 64 * LDS;
     __half* v_s = k_s + 64 * LDS;
@@ -617,7 +872,7 @@ kv8_tile_kernel(const bf16* q, const Cache cache, bf16* __restrict__ out, const 
         const uint32_t in[4] = {w.x, w.y, w.z, w.w};
         uint32_t h[8];
 #pragma unroll
-        for (int i = 0; i < 4; ++i) { h[2 * i] = kv8_halves(in[i] & 0xffffu); h[2 * i + 1] = kv8_halves(in[i] >> 16); }
+        for (int i = 0; i < 4; ++i) kv8_halves(in[i], h[2 * i], h[2 * i + 1]);
         *reinterpret_cast<uint4*>(dst) = make_uint4(h[0], h[1], h[2], h[3]);
         *reinterpret_cast<uint4*>(dst + 8) = make_uint4(h[4], h[5], h[6], h[7]);
     };
@@ -769,22 +1024,34 @@ kv8_tile_kernel(const bf16* q, const Cache cache, bf16* __restrict__ out, const 
 }
 
 template <int NG>
-int stream(const bf16* q, const Cache& cache, bf16* out, float* ws, const Kv8Step& step, int n_seqs, int max_new, int H, int G, float scale,
-           int window, int n_splits, const float* sink, int keep, const float* slopes, cudaStream_t s) {
+int stream(const bf16* q, const Cache& cache, bf16* out, void* ws, const Kv8Step& step, int n_seqs, int max_new, int H, int G, float scale,
+           int window, int n_splits, int n_ctas, const float* sink, int keep, const float* slopes, cudaStream_t s) {
     static std::atomic<unsigned long long> d0{0}, d1{0};
-    const size_t smem = stream_smem(NG);
-    const bool cluster = n_splits > 1 && !ws;
-    cudaError_t e = cluster ? plm_allow_smem(kv8_stream_kernel<NG, true>, smem, d0) : plm_allow_smem(kv8_stream_kernel<NG, false>, smem, d1);
+    const size_t smem = Few<NG>::SMEM;
+    cudaError_t e = ws ? plm_allow_smem(kv8_stream_kernel<NG, false>, smem, d1) : plm_allow_smem(kv8_stream_kernel<NG, true>, smem, d0);
     if (e != cudaSuccess) return (int)e;
-    const long tiles = ((long)max_new * (H / G) + 8 * NG - 1) / (8 * NG);
+    const long rows = (long)max_new * (H / G), tiles = (rows + 8 * NG - 1) / (8 * NG);
     if (tiles * G > 65535) return PLM_ERR_SHAPE;
-    const dim3 grid(n_splits, (unsigned)(tiles * G), n_seqs);
-    if (cluster)
-        return plm_status_of(launch_pdl_cluster(kv8_stream_kernel<NG, true>, grid, dim3(NT), dim3(n_splits, 1, 1), smem, s, q, cache, out, ws,
-                                                step, H, G, (int)tiles, scale * LOG2E, window, sink, keep, slopes));
-    return plm_status_of(launch_pdl(kv8_stream_kernel<NG, false>, grid, dim3(NT), smem, s, q, cache, out, ws, step, H, G, (int)tiles,
-                                    scale * LOG2E, window, sink, keep, slopes));
+    float* none = nullptr;
+    int2* pieces = nullptr;
+    if (!ws)
+        return plm_status_of(launch_pdl_cluster(kv8_stream_kernel<NG, true>, dim3(n_splits, (unsigned)(tiles * G), n_seqs), dim3(NT), dim3(n_splits, 1, 1),
+                                                smem, s, q, cache, out, none, pieces, step, n_seqs, H, G, (int)tiles, scale * LOG2E, window, sink, keep, slopes));
+    float* part = reinterpret_cast<float*>(ws);
+    pieces = reinterpret_cast<int2*>(part + (size_t)n_ctas * WARPS * 2 * 8 * NG * ROW);
+    int rc = plm_status_of(launch_pdl(kv8_stream_kernel<NG, false>, dim3(n_ctas), dim3(NT), smem, s, q, cache, out, part, pieces, step, n_seqs, H, G,
+                                      (int)tiles, scale * LOG2E, window, sink, keep, slopes));
+    if (rc != PLM_OK) return rc;
+    const unsigned n_walks = (unsigned)(tiles * G), n_rows = (unsigned)(rows < 8 * NG ? rows : 8 * NG);
+    if ((long)n_ctas * WARPS > 10L * n_walks * n_seqs)
+        return plm_status_of(launch_pdl(kv8_join_many_kernel<NG>, dim3(n_walks, n_rows, n_seqs), dim3(512), (size_t)n_ctas * WARPS * sizeof(float), s,
+                                        (const float*)part, (const int2*)pieces, out, step, H, G, (int)tiles, sink));
+    return plm_status_of(launch_pdl(kv8_join_kernel<NG>, dim3(n_walks, (n_rows * HD + JOIN - 1) / JOIN, n_seqs), dim3(JOIN), 0, s, (const float*)part,
+                                    (const int2*)pieces, out, step, H, G, (int)tiles, sink));
 }
+
+// (token, head) rows that a CTA of the streaming kernel takes at a time, for at most `rows` of a sequence and kv head.
+int groups_of(long rows) { return rows <= 8 ? 1 : rows <= 16 || HD > 128 ? 2 : 4; }
 
 bool bad_step(const int* tok_pos, const int* tok_seq, const int* seq_start, const int* seq_kv_len) {
     return !tok_pos != !tok_seq || !tok_pos == !seq_start || !seq_start != !seq_kv_len;
@@ -792,33 +1059,36 @@ bool bad_step(const int* tok_pos, const int* tok_seq, const int* seq_start, cons
 
 }  // namespace
 
+// CTAs that run at once, and floats of workspace for a CTA, for at most `rows` (token, head) rows of a sequence and kv head; two more
+// for every sequence, kv head and tile of that many rows.
+extern "C" int plm_kv8_few_ctas(int rows) {
+    const int ng = groups_of(rows);
+    return PLM_SM_COUNT * (ng == 1 ? (int)Few<1>::CTAS : ng == 2 ? (int)Few<2>::CTAS : (int)Few<4>::CTAS);
+}
+extern "C" int plm_kv8_few_floats(int rows) { return WARPS * 2 * 8 * groups_of(rows) * ROW; }
+extern "C" int plm_kv8_few_tile(int rows) { return 8 * groups_of(rows); }
+
 // q [n_rows, H, HD] bf16, out [n_rows, H * HD] bf16.  Either tok_pos and tok_seq [n_seqs = n_rows] (single tokens, max_new 1) or
-// seq_start [n_seqs + 1] and seq_kv_len [n_seqs].  Every sequence's keys are cut into n_splits ranges; up to eight meet in their
-// cluster where ws is null, else ws holds n_rows * H * n_splits * (HD + 2) floats.
-extern "C" int plm_kv8_attention_few(const void* q, const void* kc, const void* vc, const float* ks, const float* vs, void* out, float* ws,
+// seq_start [n_seqs + 1] and seq_kv_len [n_seqs].  With ws null every sequence's keys are cut into n_splits ranges (at most eight), which
+// meet in a cluster; else all keys of the step are dealt out to n_ctas CTAs (see the functions above for the
+// size of ws).
+extern "C" int plm_kv8_attention_few(const void* q, const void* kc, const void* vc, const float* ks, const float* vs, void* out, void* ws,
                                      const int* tok_pos, const int* tok_seq, const int* seq_start, const int* seq_kv_len,
                                      const int* block_table, int max_pages, int n_rows, int n_seqs, int max_new, int H, int G,
-                                     float scale, int window, int n_splits, const float* sink, int keep, const float* slopes,
+                                     float scale, int window, int n_splits, int n_ctas, const float* sink, int keep, const float* slopes,
                                      cudaStream_t s) {
     if (n_rows <= 0 || n_seqs <= 0 || max_new <= 0) return PLM_OK;
-    if (H <= 0 || G <= 0 || H % G || n_seqs > 65535 || n_splits < 1 || (n_splits > 1 && !ws && n_splits > MAX_CLUSTER) || n_splits > 8192 ||
-        keep < 0 || (long)n_rows * H > 0x7fffffffL)
-        return PLM_ERR_SHAPE;
+    if (H <= 0 || G <= 0 || H % G || n_seqs > 65535 || (ws ? n_ctas < 1 || n_ctas > MAX_CTAS : n_splits < 1 || n_splits > MAX_CLUSTER) || keep < 0) return PLM_ERR_SHAPE;
     if (bad_step(tok_pos, tok_seq, seq_start, seq_kv_len)) return PLM_ERR_UNSUPPORTED;
     if (((uintptr_t)q | (uintptr_t)kc | (uintptr_t)vc) & 15) return PLM_ERR_ALIGN;
-    if (n_splits == 1) ws = nullptr;
     const Kv8Step step = {tok_pos, tok_seq, seq_start, seq_kv_len, block_table, max_pages};
     const Cache cache = {(const uint8_t*)kc, (const uint8_t*)vc, ks, vs};
-    const long rows = (long)max_new * (H / G);
-    int rc;
-#define KV8_STREAM(NG_) rc = stream<NG_>((const bf16*)q, cache, (bf16*)out, ws, step, n_seqs, max_new, H, G, scale, window, n_splits, sink, keep, slopes, s)
-    if (rows <= 8) KV8_STREAM(1);
-    else if (rows <= 16 || HD > 128) KV8_STREAM(2);
-    else KV8_STREAM((HD > 128 ? 2 : 4));
-#undef KV8_STREAM
-    if (rc != PLM_OK || !ws) return rc;
-    return plm_status_of(launch_pdl(kv8_join_kernel, dim3((unsigned)((long)n_rows * H)), dim3(NT), n_splits * sizeof(float), s,
-                                    (const float*)ws, (bf16*)out, n_splits, H, sink, seq_start, n_seqs));
+    const int groups = groups_of((long)max_new * (H / G));
+    if (groups == 1) return stream<1>((const bf16*)q, cache, (bf16*)out, ws, step, n_seqs, max_new, H, G, scale, window, n_splits, n_ctas, sink, keep, slopes, s);
+    if (groups == 2) return stream<2>((const bf16*)q, cache, (bf16*)out, ws, step, n_seqs, max_new, H, G, scale, window, n_splits, n_ctas, sink, keep, slopes, s);
+    if constexpr (HD <= 128)
+        return stream<4>((const bf16*)q, cache, (bf16*)out, ws, step, n_seqs, max_new, H, G, scale, window, n_splits, n_ctas, sink, keep, slopes, s);
+    return PLM_ERR_UNSUPPORTED;
 }
 
 // The same for prompts, rows of 64 at a time: seq_start [n_seqs + 1], seq_kv_len [n_seqs], at most max_new rows a sequence.

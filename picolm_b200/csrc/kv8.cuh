@@ -18,6 +18,11 @@ __device__ __forceinline__ uint32_t kv8_halves(uint32_t two) {
     asm("{\n\t.reg .b16 h;\n\tcvt.u16.u32 h, %1;\n\tcvt.rn.f16x2.e4m3x2 %0, h;\n\t}" : "=r"(r) : "r"(two));
     return r;
 }
+// Four of them: the low two and the high two.
+__device__ __forceinline__ void kv8_halves(uint32_t four, uint32_t& lo, uint32_t& hi) {
+    asm("{\n\t.reg .b16 l, h;\n\tmov.b32 {l, h}, %2;\n\tcvt.rn.f16x2.e4m3x2 %0, l;\n\tcvt.rn.f16x2.e4m3x2 %1, h;\n\t}"
+        : "=r"(lo), "=r"(hi) : "r"(four));
+}
 __device__ __forceinline__ float2 kv8_floats(uint32_t two) {
     const uint32_t h = kv8_halves(two);
     return __half22float2(*reinterpret_cast<const __half2*>(&h));

@@ -145,17 +145,29 @@ def attention_kv8_mma_supported(q: torch.Tensor) -> bool:
 KV8_CLUSTER_SPLITS = 8          # up to this many ranges of keys meet inside a thread-block cluster, without scratch
 KV8_FEW_ROWS = 64               # (token, head) rows a sequence and kv head up to which its keys are streamed
 
-
-def kv8_row_groups(rows: int, head_dim: int) -> int:
-    """CTAs that the (token, head) rows of one sequence and kv head take in the streaming kernel (8, 16 or 32 rows each)."""
-    per = 8 if rows <= 8 else 16 if rows <= 16 or head_dim > 128 else 32
-    return -(-rows // per)
+_few = {}
 
 
-def kv8_splits(ctas: int, max_kv_len: int, head_dim: int) -> int:
-    """Into how many ranges the streaming kernel cuts the keys, for `ctas` CTAs without cutting."""
-    units = -(-max_kv_len // (32 if head_dim <= 64 else 16))
-    return max(1, min(4 * SM_COUNT // max(ctas, 1), units // 8, 512))
+def kv8_few_plan(head_dim: int, rows: int):
+    """(rows a CTA of the streaming kernel takes at a time, CTAs that run at once, floats of workspace for a CTA) for at most
+    `rows` (token, head) rows of a sequence and kv head."""
+    plan = _few.get((head_dim, rows))
+    if plan is None:
+        lib, flags = attention_variant(head_dim, "attention_kv8")
+        plan = tuple(_fn(lib, "plm_kv8_few_" + what, flags)(rows) for what in ("tile", "ctas", "floats"))
+        _few[head_dim, rows] = plan
+    return plan
+
+
+def kv8_cluster_splits(ctas: int, at_once: int, max_kv_len: int) -> int:
+    """Into how many ranges, the CTAs of a cluster, the streaming kernel cuts the keys of each sequence, for `ctas` CTAs without
+    cutting and `at_once` that run at once; 0: the keys of the step are dealt out over one wave of CTAs.  Dealing out costs a second
+    kernel and a longer start, some 6 us, and pays where the ranges would be longer than 16 pages or the CTAs more than run at once
+    (us, clusters / dealt out, 32 heads over 8: one sequence of 8,000 keys of 64 8.1 / 14.0, one of 32,000 of 128 26.6 / 24.8; 16 of 2,000
+    of 64 9.9 / 16.3, 64 of 1,000 of 128 30.1 / 27.5)."""
+    pages = -(-max_kv_len // PAGE_TOKENS)
+    splits = min(KV8_CLUSTER_SPLITS, at_once // ctas, max(1, pages // 2))
+    return splits if splits >= 1 and pages <= 16 * splits else 0
 
 
 def _attend(what, q, k_cache, v_cache, k_scale, v_scale, block_table, ints, max_new, max_kv_len, num_kv_heads, scale, window, out,
@@ -177,8 +189,8 @@ def _attend(what, q, k_cache, v_cache, k_scale, v_scale, block_table, ints, max_
             raise KernelError(f"{what}: q is on {device}, {n} on {t.device}")
     if not scale > 0:
         raise KernelError(f"{what}: the scale must be positive, got {scale}")
-    if n_splits is not None and not 1 <= n_splits <= 512:
-        raise KernelError(f"{what}: n_splits must lie in 1 .. 512, got {n_splits}")
+    if n_splits is not None and not 0 <= n_splits <= KV8_CLUSTER_SPLITS:
+        raise KernelError(f"{what}: n_splits must lie in 0 .. {KV8_CLUSTER_SPLITS}, got {n_splits}")
     decode = ints[0][1] == "tok_pos"
     _step_check(what, device, block_table, *ints)
     if decode:
@@ -213,12 +225,13 @@ def _attend(what, q, k_cache, v_cache, k_scale, v_scale, block_table, ints, max_
     lib, flags = attention_variant(hd, "attention_kv8")
     _bounds(lib, flags, k_cache, block_table, device)
     if decode or rows <= KV8_FEW_ROWS:
-        ctas = B * G * kv8_row_groups(rows, hd)
-        splits = n_splits or kv8_splits(ctas, seen, hd)
-        ws = torch.empty((T * H * splits * (hd + 2),), dtype=torch.float32, device=device) if splits > KV8_CLUSTER_SPLITS else None
+        tile, at_once, floats = kv8_few_plan(hd, rows)
+        walks = B * G * -(-rows // tile)
+        splits = kv8_cluster_splits(walks, at_once, seen) if n_splits is None else n_splits
+        ws = None if splits else torch.empty((at_once * floats + 2 * walks,), dtype=torch.float32, device=device)
         _check(_fn(lib, "plm_kv8_attention_few", flags)(
-            _p(q), *cache, _p(out), _p(ws), *step, _p(block_table), block_table.shape[1], T, B, int(max_new), H, G, *tail, splits, *rest),
-            f"{say} few splits={splits}", kernels=2 if ws is not None else 1, **need)
+            _p(q), *cache, _p(out), _p(ws), *step, _p(block_table), block_table.shape[1], T, B, int(max_new), H, G, *tail, splits, at_once, *rest),
+            f"{say} few splits={splits}", kernels=1 if splits else 2, **need)
         return out
     _check(_fn(lib, "plm_kv8_attention_tiles", flags)(
         _p(q), *cache, _p(out), *step[2:], _p(block_table), block_table.shape[1], B, int(max_new), H, G, *tail, *rest), f"{say} tiles", **need)
@@ -232,7 +245,7 @@ def attention_kv8_decode(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.
                          slopes: Optional[torch.Tensor] = None, n_splits: Optional[int] = None) -> torch.Tensor:
     """Attention of single query tokens (one per row of q [T, H, hd], at position tok_pos[t] of sequence tok_seq[t]) over the 8-bit
     cache; returns [T, H * hd].  `max_kv_len`: an upper bound of tok_pos + 1, for the choice of how many ranges the keys are cut
-    into (`n_splits` sets it).  `window`, `sink`, `keep_first`, `slopes`: see `attention_rows`."""
+    into (`n_splits` sets it: 1 to 8 ranges, or 0, all keys of the step dealt out over one wave of CTAs).  `window`, `sink`, `keep_first`, `slopes`: see `attention_rows`."""
     return _attend("attention_kv8_decode", q, k_cache, v_cache, k_scale, v_scale, block_table, ((tok_pos, "tok_pos"), (tok_seq, "tok_seq")),
                    1, max_kv_len, num_kv_heads, scale, window, out, sink, keep_first, slopes, n_splits)
 

@@ -251,7 +251,7 @@ def test_decode(case, spread, dtype):
         args["slopes"] = torch.rand(H, generator=s.g) * 0.1
     on = {k: v.to(DEV) if isinstance(v, torch.Tensor) else v for k, v in args.items()}
     order = torch.randperm(len(lens), generator=s.g).tolist()        # rows in another order than the table's
-    for splits in (None, 1, 3, 8, 11):
+    for splits in (None, 0, 1, 3, 8):
         got = ops.attention_kv8_decode(q.to(DEV), s.dk, s.dv, s.dks, s.dvs, i32([positions[b] for b in order]), i32(order), s.dt, max(lens), G,
                                        hd ** -0.5, n_splits=splits, **on)
         check_attention(got, s, q, [(t, b, positions[b]) for t, b in enumerate(order)], G, hd ** -0.5, dtype, **args)
@@ -290,10 +290,10 @@ def test_prefill(case, spread, dtype):
         args["slopes"] = torch.rand(H, generator=s.g) * 0.1
     on = {k: v.to(DEV) if isinstance(v, torch.Tensor) else v for k, v in args.items()}
     max_new = max(n for n, _ in seqs)
-    for bound in (max_new, max_new + 70):                             # an upper bound serves too
+    for bound, splits in ((max_new, None), (max_new + 70, None), (max_new, 0), (max_new, 5)):          # an upper bound serves too
         out = torch.full((T + 4, H * hd), 5.0, dtype=q.dtype, device=DEV)
         got = ops.attention_kv8_prefill(q.to(DEV), s.dk, s.dv, s.dks, s.dvs, i32(offs), i32(lens), s.dt, bound, max(lens), G, hd ** -0.5,
-                                        out=out, **on)
+                                        out=out, n_splits=splits, **on)
         assert got is out and bool((out[T:] == 5.0).all()), "rows of no sequence"
         check_attention(got, s, q, [(offs[b] + i, b, before + i) for b, (n, before) in enumerate(seqs) for i in sorted({*range(0, n, 7), n - 1} - {-1})],
                         G, hd ** -0.5, dtype, **args)
