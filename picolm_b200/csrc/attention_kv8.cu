@@ -798,6 +798,7 @@ kv8_join_many_kernel(const float* ws, const int2* pieces, bf16* __restrict__ out
 }
 
 // -------------------------------------------------------------------------------------------- prompts
+#if PLM_HD != 64 && PLM_HD != 128                // (those on tcgen05: attention_kv8_tc.cu)
 constexpr int LDS = HD + 8;                      // halves of a row in shared memory: ldmatrix without bank conflicts
 constexpr size_t TILE_SMEM = (size_t)3 * 64 * LDS * 2;
 
@@ -1023,6 +1024,8 @@ kv8_tile_kernel(const bf16* q, const Cache cache, bf16* __restrict__ out, const 
     }
 }
 
+#endif
+
 template <int NG>
 int stream(const bf16* q, const Cache& cache, bf16* out, void* ws, const Kv8Step& step, int n_seqs, int max_new, int H, int G, float scale,
            int window, int n_splits, int n_ctas, const float* sink, int keep, const float* slopes, cudaStream_t s) {
@@ -1091,6 +1094,7 @@ extern "C" int plm_kv8_attention_few(const void* q, const void* kc, const void* 
     return PLM_ERR_UNSUPPORTED;
 }
 
+#if PLM_HD != 64 && PLM_HD != 128
 // The same for prompts, rows of 64 at a time: seq_start [n_seqs + 1], seq_kv_len [n_seqs], at most max_new rows a sequence.
 extern "C" int plm_kv8_attention_tiles(const void* q, const void* kc, const void* vc, const float* ks, const float* vs, void* out,
                                        const int* seq_start, const int* seq_kv_len, const int* block_table, int max_pages, int n_seqs,
@@ -1108,3 +1112,4 @@ extern "C" int plm_kv8_attention_tiles(const void* q, const void* kc, const void
     return plm_status_of(launch_pdl(kv8_tile_kernel, grid, dim3(NT), TILE_SMEM, s, (const bf16*)q, cache, (bf16*)out, step, H, G,
                                     scale * LOG2E, window, sink, keep, slopes));
 }
+#endif

@@ -43,6 +43,7 @@ LIBRARIES: Dict[str, List[str]] = {
     "attention_tc": ["attention_tc.cu"],            # likewise, head sizes 64 and 128
     "kv8": ["kv8.cu"],
     "attention_kv8": ["attention_kv8.cu"],          # one variant per head size, as attention_mma
+    "attention_kv8_tc": ["attention_kv8_tc.cu"],    # likewise, head sizes 64 and 128
     "sampling": ["sampling.cu"],
     "recurrent": ["recurrent.cu"],
     "routed": ["routed.cu"],
@@ -61,6 +62,7 @@ VARIANTS: Dict[str, Dict[str, List[str]]] = {
     "attention_mma": {f"hd{hd}": [f"-DPLM_HD={hd}"] for hd in (64, 128)},
     "attention_tc": {f"hd{hd}": [f"-DPLM_HD={hd}"] for hd in (64, 128)},
     "attention_kv8": {f"hd{hd}": [f"-DPLM_HD={hd}"] for hd in (64, 128)},
+    "attention_kv8_tc": {f"hd{hd}": [f"-DPLM_HD={hd}"] for hd in (64, 128)},
 }
 
 

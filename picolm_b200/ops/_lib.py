@@ -105,6 +105,7 @@ _SIGNATURES = {
     "plm_kv8_append": [_vp, _vp, _vp, _i, _l, _l, _l, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _i, _vp, _vp, _vp, _i, _i, _i, _i, _i, _i, _i, _i, _vp],
     "plm_kv8_attention_rows": [_vp, _i, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _i, _i, _i, _i, _i, _i, _i, _f, _i, _i, _vp, _i, _vp, _vp],
     "plm_kv8_attention_few": [_vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _i, _i, _i, _i, _i, _i, _f, _i, _i, _i, _vp, _i, _vp, _vp],
+    "plm_kv8_attention_tc": [_vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _i, _i, _i, _i, _i, _f, _i, _vp, _vp, _i, _vp, _vp],
     "plm_kv8_few_ctas": [_i],
     "plm_kv8_few_floats": [_i],
     "plm_kv8_few_tile": [_i],
@@ -119,7 +120,8 @@ _fn_cache = {}
 # this package hand them the bounds before every launch.  An index outside its bound is then recorded in
 # the status word (`check_status` raises) instead of being followed.
 CHECKED = os.environ.get("PICOLM_B200_CHECK", "") == "1"
-CHECKED_LIBRARIES = ("elementwise", "attention_simt", "attention_mma", "attention_tc", "recurrent", "kv8", "attention_kv8")
+CHECKED_LIBRARIES = ("elementwise", "attention_simt", "attention_mma", "attention_tc", "recurrent", "kv8", "attention_kv8",
+                     "attention_kv8_tc")
 
 
 class KernelError(RuntimeError):
@@ -377,7 +379,9 @@ _WAITS = {1: "TMA producer", 2: "MMA issuer", 3: "epilogue", 4: "the CTAs' meeti
           41: "the experts' streamed weights", 42: "the experts' streamed products", 43: "the experts' streamed rows",
           51: "the experts' TMA producer", 52: "the experts' MMA issuer, results unread", 53: "the experts' MMA issuer",
           54: "the experts' epilogue", 60: "the float32 product's TMA producer", 61: "the float32 product's MMA issuer",
-          62: "the float32 product's split", 63: "the float32 product's sums"}
+          62: "the float32 product's split", 63: "the float32 product's sums",
+          70: "the 8-bit attention's MMA issuer", 71: "the 8-bit attention's conversion", 72: "the 8-bit attention's softmax",
+          73: "the 8-bit attention's pages"}
 
 
 def check_status(device="cuda:0") -> None:

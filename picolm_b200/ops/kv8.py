@@ -17,7 +17,7 @@ from typing import Optional
 import torch
 
 from ..csrc.build import attention_variant
-from ._lib import PAGE_TOKENS, SM_COUNT, KernelError, _check, _dev, _dt, _fn, _i32, _p, _stream, set_bounds
+from ._lib import PAGE_TOKENS, SM_COUNT, KernelError, _check, _dev, _dt, _fn, _i32, _p, _stream, set_bounds, status_word
 from .attention import _bias_check, _sink_check
 
 KV8_DTYPE = torch.float8_e4m3fn
@@ -232,6 +232,13 @@ def _attend(what, q, k_cache, v_cache, k_scale, v_scale, block_table, ints, max_
         _check(_fn(lib, "plm_kv8_attention_few", flags)(
             _p(q), *cache, _p(out), _p(ws), *step, _p(block_table), block_table.shape[1], T, B, int(max_new), H, G, *tail, splits, at_once, *rest),
             f"{say} few splits={splits}", kernels=1 if splits else 2, **need)
+        return out
+    if hd in (64, 128):
+        lib, flags = attention_variant(hd, "attention_kv8_tc")
+        _bounds(lib, flags, k_cache, block_table, device)
+        _check(_fn(lib, "plm_kv8_attention_tc", flags)(
+            _p(q), *cache, _p(out), *step[2:], _p(block_table), block_table.shape[1], B, int(max_new), H, G, *tail, _p(status_word(device)),
+            *rest), f"{say} tc", **need)
         return out
     _check(_fn(lib, "plm_kv8_attention_tiles", flags)(
         _p(q), *cache, _p(out), *step[2:], _p(block_table), block_table.shape[1], B, int(max_new), H, G, *tail, *rest), f"{say} tiles", **need)
