@@ -10,8 +10,8 @@
 //                  over the first half of the scores' place
 //   O += P V       tcgen05.mma, P from tensor memory, V in shared memory (MN-major); O stays in tensor memory and is scaled only when
 //                  a row's maximum outgrows its reference by 2^8 or a page's values have a scale beyond 2^6 from O's unit
-// Warps 0..7 are the softmax threads of the two tiles (quarter = warp % 4), 8..11 make halves of bytes, 12 issues the
-// MMAs and owns the tensor memory, 13 asks for pages: a page's keys and values of a kv head are contiguous, so that each is
+// Warps 0..7 are the softmax threads of the two tiles (quarter = warp % 4), 8..11 make halves of bytes, 12 and 14 issue the
+// tiles' MMAs (12 owns the tensor memory), 13 asks for pages: a page's keys and values of a kv head are contiguous, so that each is
 // one bulk copy of 4 or 8 KB into a ring of raw pages.  While one tile's threads work on page i, the tensor cores have
 // P V of the other's; the scores of a tile have two places, so that Q K^T of the next page is there when its threads
 // come for it.
@@ -195,11 +195,12 @@ kv8_tc_kernel(const bf16* q, const Cache cache, bf16* __restrict__ out, const Kv
         s_abort = 0;
         s_nan = 0;
         for (int i = 0; i < RS; ++i) { mbar_init(raw_full + 8 * i, 1); mbar_init(raw_empty + 8 * i, 128); }
-        for (int i = 0; i < KS; ++i) { mbar_init(k_full + 8 * i, 128); mbar_init(k_empty + 8 * i, 1); }
-        for (int i = 0; i < VS; ++i) { mbar_init(v_full + 8 * i, 128); mbar_init(v_empty + 8 * i, 1); }
+        for (int i = 0; i < KS; ++i) { mbar_init(k_full + 8 * i, 128); mbar_init(k_empty + 8 * i, used); }
+        for (int i = 0; i < VS; ++i) { mbar_init(v_full + 8 * i, 128); mbar_init(v_empty + 8 * i, used); }
         for (int i = 0; i < TILES; ++i) mbar_init(q_full + 8 * i, 128);
         for (int i = 0; i < 2 * TILES; ++i) { mbar_init(s_full + 8 * i, 1); mbar_init(p_ready + 8 * i, 128); mbar_init(pv_full + 8 * i, 1); }
         mbar_init(done, 1);
+        mbar_init(done + 8, 1);
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
     if (warp == 12) {
@@ -472,75 +473,67 @@ kv8_tc_kernel(const bf16* q, const Cache cache, bf16* __restrict__ out, const Kv
         if (!ok) s_abort = 1;
     } else {
         asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(OTHER_REGS));
-        if (warp == 12) {
-            // ---------------------------------------------------------- MMA issuer (the whole warp walks, one elected lane issues)
-            const uint32_t tmem_u = __shfl_sync(0xffffffffu, tmem, 0);
+        if (warp == 12 || warp == 14) {
+            // ---------------------------------------------------------- MMA issuers, one a tile (the whole warp walks, one elected lane
+            // issues).  One for both was what the tiles waited for: a page's waits, fences and issues are a chain of some 800 cycles.
+            const int t = (warp - 12) >> 1, mine = pages_of(t);
+            const uint32_t tmem_u = __shfl_sync(0xffffffffu, tmem, 0), q_at = q_smem + t * Q_BYTES;
             constexpr uint32_t idesc_s = instr_desc(BKV, false), idesc_o = instr_desc(HD, true);
-            const int pages_t[TILES] = {pages_of(0), pages_of(1)};
-            auto scores = [&](int t, int i) {                                      // S_t[i % 2] = Q_t K(i)^T
+            auto scores = [&](int i) {                                             // S[i % 2] = Q K(i)^T, and K(i)'s place is free
                 const uint32_t k_at = k_smem + (i % KS) * KV_BYTES;
                 if (elect_one()) {
 #pragma unroll
                     for (int cb = 0; cb < CB; ++cb)
 #pragma unroll
                         for (int k = 0; k < 4; ++k)
-                            mma_ss(tmem_u + TM_S + t * 128 + (i & 1) * 64, smem_desc_sw128(q_smem + t * Q_BYTES + cb * Q_BLOCK) + (uint64_t)(k * 2),
+                            mma_ss(tmem_u + TM_S + t * 128 + (i & 1) * 64, smem_desc_sw128(q_at + cb * Q_BLOCK) + (uint64_t)(k * 2),
                                    smem_desc_sw128(k_at + cb * KV_BLOCK) + (uint64_t)(k * 2), idesc_s, (cb > 0 || k > 0) ? 1u : 0u);
                     tc_commit(s_full + 16 * t + 8 * (i & 1));
+                    tc_commit(k_empty + 8 * (i % KS));
                 }
                 __syncwarp();
             };
-            auto release = [&](uint32_t bar) {
-                if (elect_one()) tc_commit(bar);
-                __syncwarp();
-            };
-            auto stopped = [&]() { return __any_sync(0xffffffffu, *(volatile int*)&s_abort); };
-            bool ok = true, issued = false;
-            for (int t = 0; t < used && ok; ++t) ok = mbar_wait_warp(q_full + 8 * t, 0, status, 70);
-            for (int i = 0; i < 2 && i < n_pages && ok; ++i) {                     // the scores' places
-                ok = mbar_wait_warp(k_full + 8 * (i % KS), (i / KS) & 1, status, 70);
-                if (!ok) break;
-                tc_fence_after();
-                for (int t = 0; t < used; ++t)
-                    if (i < pages_t[t]) scores(t, i);
-                release(k_empty + 8 * (i % KS));
-                issued = true;
-            }
-            for (int i = 0; i < n_pages && ok; ++i) {
-                const int nxt = i + 2;
-                for (int t = 0; t < used && ok; ++t) {
-                    if (i >= pages_t[t]) continue;
-                    ok = !stopped() && __all_sync(0xffffffffu, mbar_spin(p_ready + 16 * t + 8 * (i & 1), (i >> 1) & 1, status, 70));
+            auto keys = [&](int i) { return mbar_wait_warp(k_full + 8 * (i % KS), (i / KS) & 1, status, 70); };
+            auto pass = [&](uint32_t bar) { if (lane == 0) mbar_arrive(bar); };    // a page that this tile does not look at
+            bool ok = t < used;
+            if (ok) {
+                ok = mbar_wait_warp(q_full + 8 * t, 0, status, 70);
+                for (int i = 0; i < 2 && i < n_pages && ok; ++i) {                 // the scores' places
+                    ok = keys(i);
                     if (!ok) break;
                     tc_fence_after();
-                    ok = mbar_wait_warp(v_full + 8 * (i % VS), (i / VS) & 1, status, 70);
+                    if (i < mine) scores(i);
+                    else pass(k_empty + 8 * (i % KS));
+                }
+                for (int i = 0; i < n_pages && ok; ++i) {
+                    const int nxt = i + 2;
+                    ok = !*(volatile int*)&s_abort && mbar_wait_warp(v_full + 8 * (i % VS), (i / VS) & 1, status, 70) && (nxt >= n_pages || keys(nxt));
                     if (!ok) break;
-                    tc_fence_after();
-                    const uint32_t v_at = v_smem + (i % VS) * KV_BYTES, p_tm = tmem_u + TM_S + t * 128 + (i & 1) * 64;
-                    if (elect_one()) {
-#pragma unroll
-                        for (int k = 0; k < BKV / 16; ++k)                         // 16 keys a step
-                            mma_ts(tmem_u + TM_O + t * HD, p_tm + k * 8, smem_desc_sw128_mn(v_at + k * 2048), idesc_o, (i > 0 || k > 0) ? 1u : 0u);
-                        tc_commit(pv_full + 16 * t + 8 * (i & 1));
-                    }
-                    __syncwarp();
-                    // P(i) lies in the place of S(i + 2): the MMAs of one thread run in their order
-                    if (nxt < pages_t[t]) {
-                        ok = mbar_wait_warp(k_full + 8 * (nxt % KS), (nxt / KS) & 1, status, 70);
+                    if (i < mine) {
+                        ok = __all_sync(0xffffffffu, mbar_spin(p_ready + 16 * t + 8 * (i & 1), (i >> 1) & 1, status, 70));
                         if (!ok) break;
                         tc_fence_after();
-                        scores(t, nxt);
+                        const uint32_t v_at = v_smem + (i % VS) * KV_BYTES, p_tm = tmem_u + TM_S + t * 128 + (i & 1) * 64;
+                        if (elect_one()) {
+#pragma unroll
+                            for (int k = 0; k < BKV / 16; ++k)                     // 16 keys a step
+                                mma_ts(tmem_u + TM_O + t * HD, p_tm + k * 8, smem_desc_sw128_mn(v_at + k * 2048), idesc_o, (i > 0 || k > 0) ? 1u : 0u);
+                            tc_commit(pv_full + 16 * t + 8 * (i & 1));
+                            tc_commit(v_empty + 8 * (i % VS));
+                        }
+                        __syncwarp();
+                    } else {
+                        pass(v_empty + 8 * (i % VS));
                     }
+                    // P(i) lies in the place of S(i + 2): the MMAs of one thread run in their order
+                    if (nxt < mine) scores(nxt);
+                    else if (nxt < n_pages) pass(k_empty + 8 * (nxt % KS));
                 }
-                if (!ok) break;
-                release(v_empty + 8 * (i % VS));
-                if (nxt < n_pages) release(k_empty + 8 * (nxt % KS));
-            }
-            if (!ok) {
-                s_abort = 1;
-                if (issued) {                                                      // what was issued lands before the memory is given back
-                    release(done);
-                    mbar_wait_warp(done, 0, nullptr, 0);
+                if (!ok) {                                                         // what was issued lands before the memory is given back
+                    s_abort = 1;
+                    if (elect_one()) tc_commit(done + 8 * t);
+                    __syncwarp();
+                    mbar_wait_warp(done + 8 * t, 0, nullptr, 0);
                 }
             }
         } else if (warp == 13 && lane == 0) {
