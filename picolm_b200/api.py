@@ -15,11 +15,13 @@ from .sampling import SamplingParams
 
 
 def model_load(model_dir: str, dtype: str = "bfloat16", context: Optional[int] = None,
-               max_batch: int = 8, max_tokens: Optional[int] = None, device: str = "cuda:0") -> Engine:
+               max_batch: int = 8, max_tokens: Optional[int] = None, device: str = "cuda:0",
+               cache_type: Optional[str] = None) -> Engine:
     """Load a model folder (config.json + safetensors).  `context` bounds the
     length of one sequence (the reference's `-c`, default: the model's own
     limit); the cache is sized for `max_batch` sequences of that length unless
-    `max_tokens` (tokens held by all live sequences together) says otherwise."""
+    `max_tokens` (tokens held by all live sequences together) says otherwise.  `cache_type` "e4m3" holds
+    keys and values in 8 bits (the reference's `-ctk` / `-ctv`, picolm/picolm.c:140-196; see `Engine`)."""
     from .config.registry import read_config
     cfg = read_config(model_dir)
     limit = getattr(cfg, "max_position_embeddings", None) or 2048
@@ -27,7 +29,7 @@ def model_load(model_dir: str, dtype: str = "bfloat16", context: Optional[int] =
     ctx_pages = (ctx + 63) // 64 * 64
     total = max_tokens or ctx_pages * max_batch
     return Engine.from_folder(model_dir, dtype=dtype, max_tokens=total, max_seqs=max(max_batch, 1),
-                              max_seq_tokens=ctx, device=device)
+                              max_seq_tokens=ctx, device=device, cache_type=cache_type)
 
 
 def model_free(engine: Engine) -> None:

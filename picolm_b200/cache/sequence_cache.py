@@ -46,6 +46,8 @@ class KVGroup:
     pages: Dict[int, List[int]] = field(default_factory=dict)     # slot -> page of each 64-position block (0: none)
     k: Optional[torch.Tensor] = None
     v: Optional[torch.Tensor] = None
+    k_scale: Optional[torch.Tensor] = None      # float32 [layers, pages, kv_heads] where keys and values are held in 8 bits
+    v_scale: Optional[torch.Tensor] = None
     table: Optional[np.ndarray] = None          # int32 [slots, pages per sequence]: `pages` as rows, 0-padded
 
     def ordinal(self, layer: int) -> int:
@@ -61,6 +63,8 @@ class KVLayerCache:
     window: Optional[int]
     writable: bool                              # False: the layer reads another layer's cache
     keep_first: int = 0                         # first positions of a sequence that stay beside the window
+    k_scale: Optional[torch.Tensor] = None      # a cache in 8 bits: float32 [pages, G], what a page's numbers are multiplied by
+    v_scale: Optional[torch.Tensor] = None
 
 
 @dataclass
@@ -73,13 +77,15 @@ class StateLayerCache:
 class SequenceCache:
     def __init__(self, layer_specs: Sequence[Optional[CacheSpec]], max_tokens: int, max_seqs: int,
                  kv_dtype: torch.dtype = torch.bfloat16, device="cpu", max_seq_tokens: Optional[int] = None,
-                 allocate_storage: bool = True):
+                 allocate_storage: bool = True, row_dtype: Optional[torch.dtype] = None):
         """`layer_specs[i]` is what cache number i holds (None: nothing): the model numbers
         what the runs of its schedule keep, a Llama layer's keys and values being one
         such cache per run.  The indices used throughout this class are those numbers.
         `max_tokens` is the most tokens live sequences hold together, each
         sequence's count rounded up to a page; `max_seqs` the most live
-        sequences; `max_seq_tokens` the longest single sequence."""
+        sequences; `max_seq_tokens` the longest single sequence.  `kv_dtype` float8_e4m3fn: keys and values in 8 bits with a
+        scale for each page and kv head (groups without values of their own, rows that serve as key and as value, in
+        `row_dtype`, by default bfloat16)."""
         if max_tokens <= 0 or max_seqs <= 0:
             raise ValueError("max_tokens and max_seqs must be positive")
         self.max_tokens = pages_for(max_tokens) * PAGE_TOKENS
@@ -88,6 +94,8 @@ class SequenceCache:
         self.pages_per_seq = pages_for(self.max_seq_tokens)
         self.device = torch.device(device)
         self.kv_dtype = kv_dtype
+        self.in_8_bits = kv_dtype == torch.float8_e4m3fn
+        self.row_dtype = row_dtype or (torch.bfloat16 if self.in_8_bits else kv_dtype)
         self.slots = IndexPool(max_seqs, what="slot")
         self.null_slot = max_seqs                      # the state row of a step's padding sequences
         self.lengths: Dict[int, int] = {}
@@ -117,9 +125,12 @@ class SequenceCache:
         if allocate_storage:
             for g in self.kv_groups:
                 shape = (len(g.layers), n_pages + 1, g.spec.num_kv_heads, PAGE_TOKENS, g.spec.head_dim)
-                g.k = torch.zeros(shape, dtype=kv_dtype, device=self.device)
+                dtype = self.group_dtype(g)
+                g.k = torch.zeros(shape, dtype=dtype, device=self.device)
                 # a group without values of its own (a latent cache): what is kept serves as key and as value
-                g.v = torch.zeros(shape, dtype=kv_dtype, device=self.device) if g.spec.values else g.k
+                g.v = torch.zeros(shape, dtype=dtype, device=self.device) if g.spec.values else g.k
+                if self.in_8_bits and g.spec.values:
+                    g.k_scale, g.v_scale = (torch.ones(shape[:3], dtype=torch.float32, device=self.device) for _ in range(2))
             for layer, spec in self.state_specs.items():
                 self.state[layer] = torch.zeros((max_seqs + 1,) + spec.shape, dtype=_STATE_DTYPES[spec.dtype],
                                                 device=self.device)
@@ -225,7 +236,10 @@ class SequenceCache:
                 if list(row[:len(want)]) != list(want) or row[len(want):].any():
                     raise AssertionError(f"the page table row of slot {s} differs from its page list")
 
+    def group_dtype(self, g: KVGroup) -> torch.dtype:
+        return self.row_dtype if self.in_8_bits and not g.spec.values else self.kv_dtype
+
     def kv_bytes_per_token(self) -> int:
-        item = torch.empty((), dtype=self.kv_dtype).element_size()
-        return sum((2 if g.spec.values else 1) * len(g.layers) * g.spec.num_kv_heads * g.spec.head_dim * item
+        """(Without the scales of a cache in 8 bits: 8 bytes a page, kv head and layer.)"""
+        return sum((2 if g.spec.values else 1) * len(g.layers) * g.spec.num_kv_heads * g.spec.head_dim * self.group_dtype(g).itemsize
                    for g in self.kv_groups)

@@ -46,6 +46,9 @@ def build_parser() -> argparse.ArgumentParser:
     e = ap.add_argument_group("Engine options")
     e.add_argument("--dtype", default="bfloat16", choices=["bfloat16", "float32"],
                    help="bfloat16 (serving kernels) or float32 (everything in true 32-bit)")
+    e.add_argument("--cache-type", default="auto", choices=["auto", "e4m3"],
+                   help="type of the cached keys and values: auto (the run's own) or e4m3 (8 bits, a scale for each page of 64 "
+                        "tokens and kv head: half or a quarter of the cache's bytes)")
     e.add_argument("--max-batch", type=int, default=8, help="most sequences generated together (default: 8)")
     b = ap.add_argument_group("Benchmark options")
     b.add_argument("--benchmark", action="store_true",
@@ -71,7 +74,7 @@ def benchmark_context_scaling(args, base: List[int]) -> int:
 
     from . import ops
     from .api import model_load
-    engine = model_load(args.model, dtype=args.dtype, context=args.context or None, max_batch=1)
+    engine = model_load(args.model, dtype=args.dtype, context=args.context or None, max_batch=1, cache_type=args.cache_type)
     limit = engine.cache.max_seq_tokens
     n_base, chunk = len(base), max(1, args.max_tokens)
     print(f"Base prompt: {n_base} tokens", file=sys.stderr)
@@ -119,7 +122,7 @@ def benchmark_layers(args, base: List[int], iterations: int = 3) -> int:
 
     from . import ops
     from .api import model_load
-    engine = model_load(args.model, dtype=args.dtype, context=args.context or None, max_batch=1)
+    engine = model_load(args.model, dtype=args.dtype, context=args.context or None, max_batch=1, cache_type=args.cache_type)
     model = engine.model
     n_runs = len(model.spec.schedule)
     n_new = max(0, min(args.max_tokens, engine.cache.max_seq_tokens - len(base)))
@@ -213,7 +216,7 @@ def main(argv=None) -> int:
 
     from .api import generate, model_load
     engine = model_load(args.model, dtype=args.dtype, context=args.context or None,
-                        max_batch=min(args.max_batch, len(prompts)))
+                        max_batch=min(args.max_batch, len(prompts)), cache_type=args.cache_type)
     outputs, stats = generate(engine, prompts, max_tokens=args.max_tokens, temperature=args.temperature,
                               top_p=args.top_p, top_k=args.top_k, min_p=args.min_p, seed=args.seed,
                               stop_ids=args.stop_ids, return_stats=True)

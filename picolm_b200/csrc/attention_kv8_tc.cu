@@ -166,12 +166,14 @@ kv8_tc_kernel(const bf16* q, const Cache cache, bf16* __restrict__ out, const Kv
     __shared__ int s_abort, s_nan;
 
     pdl_wait();
-    const int g = blockIdx.y, R = H / G;
+    // CTAs start in the order of their index: the longest tiles of all kv heads first, the short ones fill the end
+    const unsigned lin = blockIdx.y * gridDim.x + blockIdx.x;
+    const int g = lin % G, rank = lin / G, R = H / G;
     const Kv8Seq sq = kv8_seq(step, blockIdx.z);
     const long n_rows = (long)sq.n_new * R;
     const int n_tiles = (int)((n_rows + TILES * BQ - 1) / (TILES * BQ));
-    if ((int)blockIdx.x >= n_tiles) return;
-    const long row0 = (long)(n_tiles - 1 - blockIdx.x) * (TILES * BQ);             // the longest tiles first
+    if (rank >= n_tiles) return;
+    const long row0 = (long)(n_tiles - 1 - rank) * (TILES * BQ);
     const int rows = (int)min((long)TILES * BQ, n_rows - row0);
     const int used = rows > BQ ? 2 : 1;                                            // tiles that have rows
     const int pos_first = sq.pos0 + (int)(row0 / R), pos_last = sq.pos0 + (int)((row0 + rows - 1) / R);
@@ -265,9 +267,11 @@ kv8_tc_kernel(const bf16* q, const Cache cache, bf16* __restrict__ out, const Kv
         float m_ref = -INFINITY, l = 0.f;
         int eo = 0;
         bool ok = true;
-        float ks_next = 0.f, vs_next = 1.f;                                        // the page's scales, a page ahead
+        float ks_next = 0.f, vs_next = 1.f;                                        // the page's scales, a page ahead,
+        int page_next = 0;                                                         // and the number of the page after it
         if (my_pages > 0) {
             const size_t at = (size_t)PLM_PAGE_NO(sq.pages[page_at(0)]) * G + g;
+            page_next = sq.pages[page_at(min(1, my_pages - 1))];
             ks_next = cache.ks[at];
             vs_next = cache.vs[at];
             eo = kv8_exponent_of_scale(vs_next);
@@ -276,9 +280,10 @@ kv8_tc_kernel(const bf16* q, const Cache cache, bf16* __restrict__ out, const Kv
             const float c = c_row * ks_next;
             const int ev = kv8_exponent_of_scale(vs_next);
             if (i + 1 < my_pages) {
-                const size_t at = (size_t)PLM_PAGE_NO(sq.pages[page_at(i + 1)]) * G + g;
+                const size_t at = (size_t)PLM_PAGE_NO(page_next) * G + g;
                 ks_next = cache.ks[at];
                 vs_next = cache.vs[at];
+                page_next = sq.pages[page_at(min(i + 2, my_pages - 1))];
             }
             const uint32_t s_tm = tmem + lanes + TM_S + t * 128 + (i & 1) * 64;
             if (!mbar_spin(s_full + 16 * t + 8 * (i & 1), (i >> 1) & 1, status, 72)) { ok = false; break; }

@@ -721,7 +721,8 @@ extern "C" int plm_add_bias(float* x, const float* bias, int n_rows, int d, cuda
 //   the leading rot_dim components of every head of q and k are rotated by the token's position
 //   (pairing 0: (x[i], x[i + rot_dim/2]); pairing 1: (x[2i], x[2i+1])), the others pass
 //   v += bias_v
-// Queries go to q_out [T, H, hd_c], keys and values into the paged cache [pages, G, PLM_PAGE, hd_c]; hd_c >= D, Dv
+// Queries go to q_out [T, H, hd_c], keys and values into the paged cache [pages, G, PLM_PAGE, hd_c] (without a block_table into
+// rows [T, G, hd_c]: a cache in 8 bits takes them from there); hd_c >= D, Dv
 // is the one head size of the cache and of the attention kernels, and what lies beyond a head's own width is
 // written as zero (a zero component adds nothing to a score; a zero value column is multiplied by zero weights of
 // the output projection).  One block per token; the token's q and k sit in shared memory between the sums of
@@ -842,14 +843,15 @@ qk_norm_rope_store_kernel(const Ta* qkv, const float* bias, const Tw* wq,
         sk = block_sum<NT>(sk, red);
         if (wk && !per_head) rk = 1.0f / sqrtf(sk / (float)nk + eps);
     }
-    size_t page_base = 0;
-    int in_page = 0;
-    bool have_page = false;
-    if (own_kv) {
+    // where a key or value head's row goes: its place in the head's part of the page, or (no block_table) row (t, head) of [T, G, hd_c]
+    size_t kv_row = (size_t)t * G;
+    int kv_step = 1;
+    bool have_page = own_kv != 0;
+    if (own_kv && block_table) {
         const int page = PLM_PAGE_NO(block_table[(size_t)PLM_SEQ_NO(tok_seq[t]) * max_pages + pos / PLM_PAGE]);
         have_page = page >= 0;
-        page_base = (size_t)(page < 0 ? 0 : page) * G;
-        in_page = pos % PLM_PAGE;
+        kv_row = (size_t)(page < 0 ? 0 : page) * G * PLM_PAGE + pos % PLM_PAGE;
+        kv_step = PLM_PAGE;
     }
     const int rot_half = rot_dim / 2, half_c = hd_c / 2;
     const int heads = H + (own_kv ? G : 0);
@@ -877,7 +879,7 @@ qk_norm_rope_store_kernel(const Ta* qkv, const float* bias, const Tw* wq,
             o = q_out + ((size_t)t * H + hh) * hd_c;
         } else {
             if (!have_page) continue;
-            o = kc + ((page_base + hh) * PLM_PAGE + in_page) * hd_c;
+            o = kc + (kv_row + (size_t)hh * kv_step) * hd_c;
         }
         for (int j = lane; j < half_c; j += 32) {
             int ia, ib;
@@ -914,7 +916,7 @@ qk_norm_rope_store_kernel(const Ta* qkv, const float* bias, const Tw* wq,
                 v = batched ? qk_sm[nq + nk + g * Dv + c] : column(nq + nk + g * Dv + c);
                 if (bias) v += bias[nq + nk + g * Dv + c];
             }
-            vc[((page_base + g) * PLM_PAGE + in_page) * hd_c + c] = from_f32<Tc>(v);
+            vc[(kv_row + (size_t)g * kv_step) * hd_c + c] = from_f32<Tc>(v);
         }
     }
 }

@@ -70,7 +70,7 @@ __device__ __forceinline__ Kv8Seq kv8_seq(const Kv8Step& s, int b) {
     } else {
         q.t0 = s.seq_start[b];
         q.n_new = s.seq_start[b + 1] - q.t0;
-        q.pos0 = PLM_POSITION(s.seq_kv_len[b] - 1) + 1 - q.n_new;
+        q.pos0 = q.n_new > 0 ? PLM_POSITION(s.seq_kv_len[b] - 1) + 1 - q.n_new : 0;
         q.pages = s.block_table + (size_t)b * s.max_pages;
     }
     return q;

@@ -24,24 +24,46 @@ from .model import Model
 from .step_batch import StepShape, build_step_batch
 
 
+CACHE_TYPES = ("auto", "e4m3")
+
+
+def cache_dtype_of(name: Optional[str], run: torch.dtype) -> torch.dtype:
+    """The element type of the cache: None or "auto" the run's own, "e4m3" 8 bits with a scale for each page and kv head."""
+    if name is None or name == "auto":
+        return run
+    if name == "e4m3":
+        return torch.float8_e4m3fn
+    raise ValueError(f"cache type {name!r} is not supported ({', '.join(CACHE_TYPES)})")
+
+
 class Engine:
     def __init__(self, model: Model, max_tokens: int, max_seqs: Optional[int] = None,
-                 max_seq_tokens: Optional[int] = None, use_graphs: Optional[bool] = None):
+                 max_seq_tokens: Optional[int] = None, use_graphs: Optional[bool] = None, cache_type: Optional[str] = None):
         """`max_tokens`: the most tokens that live sequences hold at any time, each
         sequence's count rounded up to a multiple of the page size.  `max_seqs`:
         the most sequences alive at once (default: one per page).
         `max_seq_tokens`: the longest single sequence (default: the model's
-        position limit, or the whole cache if that is smaller)."""
+        position limit, or the whole cache if that is smaller).  `cache_type`: "auto" (None), keys and values in the run's
+        type, or "e4m3", in 8 bits with a scale for each page of 64 tokens and kv head (rows of a latent cache and states stay in
+        their types)."""
         if not model.loaded:
             raise RuntimeError("the model has no weights yet")
         self.model = model
         self.runtime = model.runtime
         spec = model.spec
         longest = min(max_seq_tokens or spec.max_positions, spec.max_positions)
+        kv_dtype = cache_dtype_of(cache_type, self.runtime.dtype)
+        if kv_dtype != self.runtime.dtype:
+            for block in model.blocks:
+                for prefix, part in block.parts():
+                    specs = part.cache_specs() if hasattr(part, "cache_specs") else [part.cache_spec()] if hasattr(part, "cache_spec") else []
+                    if any(sp is not None and sp.kind == "kv" and sp.values for sp in specs) and not part.takes_kv8:
+                        raise ValueError(f"cache type {cache_type!r}: the {part.family} {part.kind!r} keeps keys and values that this "
+                                         f"cache does not take (heads of a multiple of 8 up to 256, written by a part that says takes_kv8)")
         self.cache = SequenceCache(model.cache_specs(), max_tokens=max_tokens,
                                    max_seqs=max_seqs or max(1, (max_tokens + 63) // 64),
-                                   kv_dtype=self.runtime.dtype, device=self.runtime.device,
-                                   max_seq_tokens=longest)
+                                   kv_dtype=kv_dtype, device=self.runtime.device,
+                                   max_seq_tokens=longest, row_dtype=self.runtime.dtype)
         model.prepare(self.cache.max_seq_tokens)
         self.vocab_size = spec.vocab_size
         # Decode steps replay a CUDA graph when every part of every block says that its forward only
@@ -147,14 +169,14 @@ class Engine:
     @staticmethod
     def from_folder(model_dir: str, dtype="bfloat16", max_tokens: int = 4096, max_seqs: Optional[int] = None,
                     max_seq_tokens: Optional[int] = None, device="cuda:0",
-                    use_graphs: Optional[bool] = None) -> "Engine":
+                    use_graphs: Optional[bool] = None, cache_type: Optional[str] = None) -> "Engine":
         """Load `model_dir` (config.json + safetensors); the model class is chosen
         by config.json's `architectures` through the registry."""
         runtime = Runtime.create(dtype, device)
         config = read_config(model_dir)
         model = Model(spec_of(config), runtime)
         load_weights(model, model_dir)
-        eng = Engine(model, max_tokens, max_seqs, max_seq_tokens, use_graphs=use_graphs)
+        eng = Engine(model, max_tokens, max_seqs, max_seq_tokens, use_graphs=use_graphs, cache_type=cache_type)
         eng.config = config
         return eng
 

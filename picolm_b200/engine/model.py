@@ -156,8 +156,8 @@ class Model:
                 gi = cache.layer_group[c]
                 g = cache.kv_groups[gi]
                 o = g.ordinal(c)
-                out.append(KVLayerCache(g.k[o], g.v[o], step.block_tables[gi], g.spec.window, writable,
-                                        g.spec.keep_first))
+                out.append(KVLayerCache(g.k[o], g.v[o], step.block_tables[gi], g.spec.window, writable, g.spec.keep_first,
+                                        None if g.k_scale is None else g.k_scale[o], None if g.v_scale is None else g.v_scale[o]))
             else:
                 out.append(StateLayerCache(cache.state[c], writable))
         return out

@@ -219,10 +219,11 @@ def attention_decode(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tens
 
 class _MaskedView:
     """A `KVLayerCache` seen through another mask: `window` holds the kernels' number (`key_mask`)."""
-    __slots__ = ("k", "v", "block_table", "window", "writable", "keep_first")
+    __slots__ = ("k", "v", "block_table", "window", "writable", "keep_first", "k_scale", "v_scale")
 
     def __init__(self, kv, mask: int):
         self.k, self.v, self.block_table, self.window, self.writable = kv.k, kv.v, kv.block_table, mask, kv.writable
+        self.k_scale, self.v_scale = getattr(kv, "k_scale", None), getattr(kv, "v_scale", None)
         self.keep_first = 0
 
 
@@ -295,6 +296,14 @@ def attention(q: torch.Tensor, kv, step, num_kv_heads: int, scale: float, chunk:
     more = dict(sink=sink, slopes=slopes, keep_first=int(getattr(kv, "keep_first", 0) or 0))
     if chunk:
         kv = _MaskedView(kv, key_mask(kv.window, chunk))
+    if getattr(kv, "k_scale", None) is not None:             # a cache in 8 bits
+        from .kv8 import attention_kv8_decode, attention_kv8_prefill
+        cache = (kv.k, kv.v, kv.k_scale, kv.v_scale)
+        if step.is_decode:
+            return attention_kv8_decode(q, *cache, step.tok_pos, step.tok_seq, kv.block_table, step.max_position + 1, num_kv_heads, scale,
+                                        window=kv.window, **more)
+        return attention_kv8_prefill(q, *cache, step.seq_start, step.seq_kv_len, kv.block_table, step.max_new, step.max_position + 1,
+                                     num_kv_heads, scale, window=kv.window, **more)
     if attention_mma_supported(q):
         if step.is_decode:
             splits = decode_splits(q.shape[0], q.shape[1], num_kv_heads, step.max_position + 1, q.shape[2])

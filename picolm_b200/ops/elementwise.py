@@ -316,7 +316,7 @@ def qk_norm_rope_store(qkv: torch.Tensor, bias: Optional[torch.Tensor], q_norm: 
     its scores.  `conv` (float32 [taps, columns of qkv], tap-major, the token's own tap last; no bias with it): every
     column is first convolved over time with the sequence's projected rows before; `conv_state` (float32 [slots + 1,
     >= (taps - 1) * columns], contiguous rows) holds every sequence's last taps - 1 projected rows, oldest first, and
-    is brought up to date."""
+    is brought up to date.  A cache in 8 bits (`kv.k_scale`) takes the keys and values by a kernel of its own behind this one."""
     if not qkv.is_cuda or qkv.dim() != 2 or qkv.stride(1) != 1:
         raise KernelError("qk_norm_rope_store: qkv must be a matrix with contiguous rows on the device")
     _dev(q_out, "q_out")
@@ -329,7 +329,12 @@ def qk_norm_rope_store(qkv: torch.Tensor, bias: Optional[torch.Tensor], q_norm: 
     cols = H * D + ((G * D + (0 if values_from_keys else G * Dv)) if own_kv else 0)
     if qkv.shape != (T, cols) or q_out.shape != (T, H, hd_c):
         raise KernelError("qk_norm_rope_store: qkv / q_out shapes do not match the head counts")
-    if own_kv:
+    in_8_bits = own_kv and getattr(kv, "k_scale", None) is not None
+    k_to, v_to, table = kv.k, kv.v, kv.block_table
+    if in_8_bits:                                            # rows first, then into the cache: a page's scale goes by all of them
+        k_to, v_to = (torch.empty((T, G, hd_c), dtype=q_out.dtype, device=q_out.device) for _ in range(2))
+        table = None
+    elif own_kv:
         for c, n in ((kv.k, "k_cache"), (kv.v, "v_cache")):
             _dev(c, n)
             if c.dtype != q_out.dtype or c.shape[1:] != (G, PAGE_TOKENS, hd_c):
@@ -355,7 +360,7 @@ def qk_norm_rope_store(qkv: torch.Tensor, bias: Optional[torch.Tensor], q_norm: 
         if wn is not None and (wn.dtype != q_out.dtype or wn.shape != (size,) or not wn.is_cuda):
             raise KernelError(f"qk_norm_rope_store: {n} must be [{size}] of {q_out.dtype}")
     if (rotation is None or rotation.cos is None) and bias is None and q_norm is None and k_norm is None and q_scale is None \
-            and conv is None and own_kv and not values_from_keys and qkv.dtype == q_out.dtype:
+            and conv is None and own_kv and not in_8_bits and not values_from_keys and qkv.dtype == q_out.dtype:
         per = 16 // qkv.element_size()
         if not (D % per or Dv % per or hd_c % per or qkv.stride(0) % per or qkv.data_ptr() % 16):
             # nothing is done to the rows on their way: 16 bytes at a time
@@ -378,14 +383,17 @@ def qk_norm_rope_store(qkv: torch.Tensor, bias: Optional[torch.Tensor], q_norm: 
                n_positions=kv.block_table.shape[1] * PAGE_TOKENS, device=qkv.device)
     _check(_fn("elementwise", "plm_qk_norm_rope_store")(
         _p(qkv), _dt(qkv, "qkv"), _p(bias), _p(q_norm), _p(k_norm) if own_kv else None, float(eps), _p(q_out),
-        _p(kv.k) if own_kv else None, _p(kv.v) if own_kv else None, _dt(q_out, "q_out"), _p(cos), _p(sin),
-        _p(step.tok_pos), _p(step.tok_seq), _p(kv.block_table), kv.block_table.shape[1], T, H, G, D, Dv, hd_c, rot,
+        _p(k_to) if own_kv else None, _p(v_to) if own_kv else None, _dt(q_out, "q_out"), _p(cos), _p(sin),
+        _p(step.tok_pos), _p(step.tok_seq), _p(table), kv.block_table.shape[1], T, H, G, D, Dv, hd_c, rot,
         0 if pairing == "half" else 1, 1 if own_kv else 0, 1 if per_head else 0, 1 if values_from_keys else 0,
         qkv.stride(0), _p(q_scale), _p(conv), taps, _p(conv_state) if conv is not None else None, lds,
         _p(step.seq_start) if conv is not None else None, _p(step.seq_slot) if conv is not None else None,
         step.n_seqs if conv is not None else 0, 1 if conv is not None and step.is_decode else 0, _stream()),
         f"qk_norm_rope_store T={T}", kernels=2 if conv is not None and taps > 1 and not (step.is_decode and step.n_seqs == T) else 1,
         nbytes=qkv.numel() * qkv.element_size() + T * (H + (2 * G if own_kv else 0)) * hd_c * q_out.element_size())
+    if in_8_bits:
+        from .kv8 import store_kv8
+        store_kv8(k_to, v_to, kv.k, kv.v, kv.k_scale, kv.v_scale, step.seq_start, step.seq_kv_len, kv.block_table, step.max_new)
 
 
 def _f32_vec(t: Optional[torch.Tensor], name: str, d: int) -> None:

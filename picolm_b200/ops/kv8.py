@@ -143,7 +143,7 @@ def attention_kv8_mma_supported(q: torch.Tensor) -> bool:
 
 
 KV8_CLUSTER_SPLITS = 8          # up to this many ranges of keys meet inside a thread-block cluster, without scratch
-KV8_FEW_ROWS = 64               # (token, head) rows a sequence and kv head up to which its keys are streamed
+KV8_FEW_ROWS, KV8_FEW_ROWS_MOST = 64, 256          # (token, head) rows a sequence and kv head up to which keys may be streamed
 
 _few = {}
 
@@ -168,6 +168,21 @@ def kv8_cluster_splits(ctas: int, at_once: int, max_kv_len: int) -> int:
     pages = -(-max_kv_len // PAGE_TOKENS)
     splits = min(KV8_CLUSTER_SPLITS, at_once // ctas, max(1, pages // 2))
     return splits if splits >= 1 and pages <= 16 * splits else 0
+
+
+def kv8_streams(walks: int, rows: int, max_kv_len: int, head_dim: int) -> bool:
+    """Whether prompts of at most `rows` (token, head) rows a sequence and kv head, `walks` of those, have their keys streamed (32 rows
+    at a time, the keys cut among CTAs) or take a CTA for 256 rows that walks all of them.  By what the two take a page: the tcgen05
+    kernel about 1 us whatever the rows, the streaming one 0.9 us of an SM for 32 rows of heads of 128 (0.4 of 64) and 10 more to begin
+    and join.  us, streamed / not, 32 heads over 8 of 128: 16 sequences of 9 tokens behind 3,000 75 / 49; one of 4, 16 and 40 behind
+    8,000 16 / 106, 53 / 106, 79 / 144."""
+    if head_dim not in (64, 128):
+        return rows <= KV8_FEW_ROWS
+    if rows > KV8_FEW_ROWS_MOST:
+        return False
+    pages = -(-max_kv_len // PAGE_TOKENS)
+    streamed = 10 + walks * -(-rows // 32) * pages * (0.9 if head_dim == 128 else 0.4) / SM_COUNT
+    return streamed < -(-walks // SM_COUNT) * pages
 
 
 def _attend(what, q, k_cache, v_cache, k_scale, v_scale, block_table, ints, max_new, max_kv_len, num_kv_heads, scale, window, out,
@@ -224,7 +239,7 @@ def _attend(what, q, k_cache, v_cache, k_scale, v_scale, block_table, ints, max_
         return out
     lib, flags = attention_variant(hd, "attention_kv8")
     _bounds(lib, flags, k_cache, block_table, device)
-    if decode or rows <= KV8_FEW_ROWS:
+    if decode or kv8_streams(B * G, rows, seen, hd):
         tile, at_once, floats = kv8_few_plan(hd, rows)
         walks = B * G * -(-rows // tile)
         splits = kv8_cluster_splits(walks, at_once, seen) if n_splits is None else n_splits

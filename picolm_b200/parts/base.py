@@ -71,6 +71,9 @@ class Part:
     # host, not even `step.slots` or `step.new_lens` (they are None in a captured step), and rows that belong to no
     # sequence (padding) may hold anything.  Steps with prompts replay graphs only if every part says so.
     graph_safe_prompts: bool = False
+    # Whether the part writes and reads keys and values that the cache holds in 8 bits (`KVLayerCache.k_scale`).  An engine with
+    # such a cache asks it of every part that keeps keys and values.
+    takes_kv8: bool = False
     # Whether forward() runs a step with prompts in different ways by what its sequences bring (`step.shape`).  `step_route`
     # then says in which, and a captured step is replayed only for shapes with the same answer.
     chooses_by_shape: bool = False

@@ -80,6 +80,12 @@ class Attention(Part):
     def graph_safe_prompts(self) -> bool:
         return bool(getattr(self.position, "graph_safe_prompts", False))
 
+    @property
+    def takes_kv8(self) -> bool:
+        """Keys and values may be held in 8 bits: heads of a size that cache takes, and a position encoding that writes it (in the
+        general form keys and values go in by a kernel of their own)."""
+        return ops.kv8_supported(self.hd_c) and (self.general or bool(getattr(self.position, "takes_kv8", False)))
+
     def __init__(self, params, runtime):
         super().__init__(params, runtime)
         p = self.params
@@ -328,6 +334,11 @@ class ParallelMixers(Part):
     @property
     def graph_safe_prompts(self) -> bool:
         return all(bool(getattr(part, "graph_safe_prompts", False)) for _, part in self.halves)
+
+    @property
+    def takes_kv8(self) -> bool:
+        return all(bool(getattr(part, "takes_kv8", False)) for _, part in self.halves
+                   if part.cache_spec() is not None and part.cache_spec().kind == "kv" and part.cache_spec().values)
 
     @property
     def chooses_by_shape(self) -> bool:

@@ -5,7 +5,8 @@ values go into the cache.
 Interface of the family: `prepare(n_positions)` once before the first step, and
 `apply(qkv, q_out, kv, step, num_heads, num_kv_heads, head_dim)`, which must fill
 `q_out` [T, H, hd] and, if `kv.writable`, write this step's keys and values into
-`kv.k` / `kv.v` at each token's (sequence, position).
+`kv.k` / `kv.v` at each token's (sequence, position).  One that can write a cache in 8 bits (`kv.k_scale`, `kv.v_scale`) says
+`takes_kv8`.
 
 RoPE as the reference builds and applies it: `theta(p, i) = p / base^(2i/rot)`,
 `(x0, x1) -> (x0 cos - x1 sin, x0 sin + x1 cos)`, queries and keys only
@@ -85,6 +86,7 @@ class RotaryEncoding(Part):
     """params: head_dim, rotary_dim, theta, scaling (dict or None), pairing
     ("half" or "adjacent"), max_positions."""
 
+    takes_kv8 = True
     graph_safe = True
     graph_safe_prompts = True
 
@@ -120,6 +122,11 @@ class RotaryEncoding(Part):
             raise RuntimeError(
                 f"position {step.max_position} lies beyond the rotary table; call prepare() with the cache's "
                 f"longest sequence first")
+        if kv.writable and getattr(kv, "k_scale", None) is not None:
+            ops.rope_store_kv8(qkv, q_out, kv.k, kv.v, kv.k_scale, kv.v_scale, self.cos, self.sin, step.seq_start, step.seq_kv_len,
+                               kv.block_table, step.max_new, num_heads, num_kv_heads, head_dim, self.params["rotary_dim"],
+                               self.params["pairing"])
+            return
         ops.rope_store(qkv, q_out, kv.k, kv.v, self.cos, self.sin, step.tok_pos, step.tok_seq, kv.block_table,
                        num_heads, num_kv_heads, head_dim, self.params["rotary_dim"], self.params["pairing"],
                        store=kv.writable)
@@ -129,6 +136,7 @@ class RotaryEncoding(Part):
 class NoPositionEncoding(Part):
     """Queries and keys go through unrotated."""
 
+    takes_kv8 = True
     graph_safe = True
     graph_safe_prompts = True
 
@@ -136,5 +144,9 @@ class NoPositionEncoding(Part):
         pass
 
     def apply(self, qkv, q_out, kv, step, num_heads, num_kv_heads, head_dim) -> None:
+        if kv.writable and getattr(kv, "k_scale", None) is not None:
+            ops.rope_store_kv8(qkv, q_out, kv.k, kv.v, kv.k_scale, kv.v_scale, None, None, step.seq_start, step.seq_kv_len,
+                               kv.block_table, step.max_new, num_heads, num_kv_heads, head_dim, 0, "half")
+            return
         ops.rope_store(qkv, q_out, kv.k, kv.v, None, None, step.tok_pos, step.tok_seq, kv.block_table,
                        num_heads, num_kv_heads, head_dim, 0, "half", store=kv.writable)
