@@ -24,6 +24,7 @@ struct Append {
 
 template <typename T, int N> struct Pack;
 template <> struct Pack<float, 4> { typedef float4 type; };
+template <> struct Pack<bf16, 8> { typedef uint4 type; };
 template <> struct Pack<bf16, 4> { typedef uint2 type; };
 template <> struct Pack<float, 1> { typedef float type; };
 template <> struct Pack<bf16, 1> { typedef uint16_t type; };
@@ -44,8 +45,8 @@ template <typename T, int N> __device__ __forceinline__ void store_group(T* p, c
     *reinterpret_cast<P*>(p) = w;
 }
 
-// A unit is 2 * N numbers of one row: N pairs of the rotation, or 2 * N numbers in a row that are not rotated.  N is 4 where the
-// rotated part of a head is a multiple of 8 numbers (loads of 8 or 16 bytes, stores of 4 to the cache), else 1.
+// A unit is 2 * N numbers of one row: N pairs of the rotation, or 2 * N numbers in a row that are not rotated.  N numbers lie together and
+// are one load: 16 bytes where the rotated part of a head and the head are multiples of 2 N, 8 bytes or one number where not.
 template <int N> struct Unit {
     int ia, ib;                                  // where its first and its second N numbers lie in the head
     int angle;                                   // its first pair's column of the tables, -1: not rotated
@@ -56,45 +57,57 @@ template <int N> struct Unit {
         angle = turned ? N * u : -1;
     }
 };
-template <int N>
-__device__ __forceinline__ void turn(float* x, const Append& a, const Unit<N>& u, int pos) {
-    if (u.angle < 0) return;
-    const size_t at = (size_t)min(pos, a.n_table - 1) * (a.rot / 2) + u.angle;
+template <int N> struct Angles {
     float c[N], s[N];
-    load_group<float, N>(a.cos_t + at, c);
-    load_group<float, N>(a.sin_t + at, s);
-    if (a.pairing == 0) {
+    __device__ __forceinline__ void load(const Append& a, const Unit<N>& u, int pos) {
+        if (u.angle < 0) return;
+        const size_t at = (size_t)min(pos, a.n_table - 1) * (a.rot / 2) + u.angle;
+        constexpr int M = N < 4 ? N : 4;
 #pragma unroll
-        for (int i = 0; i < N; ++i) {
-            const float p = x[i], q = x[N + i];
-            x[i] = rope_first(p, q, c[i], s[i]);
-            x[N + i] = rope_second(p, q, c[i], s[i]);
-        }
-    } else {
-#pragma unroll
-        for (int i = 0; i < N; ++i) {
-            const float p = x[2 * i], q = x[2 * i + 1];
-            x[2 * i] = rope_first(p, q, c[i], s[i]);
-            x[2 * i + 1] = rope_second(p, q, c[i], s[i]);
+        for (int i = 0; i < N; i += M) {
+            load_group<float, M>(a.cos_t + at + i, c + i);
+            load_group<float, M>(a.sin_t + at + i, s + i);
         }
     }
-}
+    __device__ __forceinline__ void turn(float* x, const Append& a, const Unit<N>& u) const {
+        if (u.angle < 0) return;
+        if (a.pairing == 0) {
+#pragma unroll
+            for (int i = 0; i < N; ++i) {
+                const float p = x[i], q = x[N + i];
+                x[i] = rope_first(p, q, c[i], s[i]);
+                x[N + i] = rope_second(p, q, c[i], s[i]);
+            }
+        } else {
+#pragma unroll
+            for (int i = 0; i < N; ++i) {
+                const float p = x[2 * i], q = x[2 * i + 1];
+                x[2 * i] = rope_first(p, q, c[i], s[i]);
+                x[2 * i + 1] = rope_second(p, q, c[i], s[i]);
+            }
+        }
+    }
+};
 
-// An item is one head's rows of the step that lie on one page: a query head's are rotated, a key or value head's decide with what
-// the page already holds about its scale and go in.  W warps an item: 8 for prompts (an item is up to 64 rows, a CTA; what a
-// thread loads stays in its registers until the scale is known), 1 for a few tokens a sequence (four items a CTA).
+// An item is the rows of the step that lie on one page, of one key or value head (they decide with what the page already holds about its
+// scale and go in) or of Q_HEADS query heads (which share the angles: a table's row is as long as a head's).  W warps an item: 4 or 8 for
+// prompts (an item is up to 64 rows, a CTA; what a thread loads stays in its registers until the scale is known), 1 for a few
+// tokens a sequence (four items a CTA).  EVEN: a row's units divide the item's threads, so that a thread has one place in a row
+// and every so many rows (no division on the way).
 // One read of the projection, one write of what it becomes: bound by memory for prompts, by the launch for single tokens.
-constexpr int HELD = 4;                          // units that a thread keeps between the two passes; more are read again (from L1)
-template <typename T, int N, int W>
+constexpr int Q_HEADS = 4;
+template <int N> struct Held { enum : int { UNITS = N == 8 ? 2 : 4 }; };      // units that a thread keeps between the two passes; more are read again
+template <typename T, int N, int W, bool EVEN>
 __global__ void __launch_bounds__(W == 1 ? 128 : 32 * W)
 kv8_append_kernel(const Append a) {
     pdl_wait();
     pdl_launch_dependents();
-    constexpr int ITEMS = W == 1 ? 4 : 1, S = 32 * W, KEEP = W == 1 ? 1 : HELD;
-    const int head = blockIdx.y * ITEMS + (W == 1 ? threadIdx.x >> 5 : 0);
+    constexpr int ITEMS = W == 1 ? 4 : 1, S = 32 * W, KEEP = W == 1 ? 1 : (int)Held<N>::UNITS;
+    const int q_items = (a.H + Q_HEADS - 1) / Q_HEADS;
+    const int item = blockIdx.y * ITEMS + (W == 1 ? threadIdx.x >> 5 : 0);
     const int tid = W == 1 ? threadIdx.x & 31 : threadIdx.x;
     const int b = blockIdx.z;
-    if (head >= a.H + 2 * a.G) return;
+    if (item >= q_items + 2 * a.G) return;
     const int t0 = a.seq_start[b], n_new = a.seq_start[b + 1] - t0;
     if (n_new <= 0) return;
     const int pos0 = PLM_POSITION(a.seq_kv_len[b] - 1) + 1 - n_new;
@@ -103,36 +116,42 @@ kv8_append_kernel(const Append a) {
     if (rows <= 0) return;
     const int units = a.hd / (2 * N), total = rows * units;
     const int t_first = t0 + first - pos0;                       // the token of the item's first row
+    const int u0 = EVEN ? tid % units : 0, r0 = EVEN ? tid / units : 0, r_step = EVEN ? S / units : 0;
+    // the thread's j-th unit: its row and its place in the row
+    auto row_of = [&](int j) { return EVEN ? r0 + j * r_step : (tid + j * S) / units; };
+    auto place_of = [&](int j) { return EVEN ? u0 : (tid + j * S) % units; };
+    const int mine = tid < total ? (total - tid + S - 1) / S : 0;
 
-    if (head < a.H) {
-        const T* src = reinterpret_cast<const T*>(a.q_in) + (size_t)head * a.hd;
-        T* dst = reinterpret_cast<T*>(a.q_out) + ((size_t)t_first * a.H + head) * a.hd;
-        for (int base = tid; base < total; base += KEEP * S) {
-            float x[KEEP][2 * N];
+    if (item < q_items) {
+        const int h0 = item * Q_HEADS, heads = min(Q_HEADS, a.H - h0);
+        const T* src = reinterpret_cast<const T*>(a.q_in) + (size_t)h0 * a.hd;
+        T* dst = reinterpret_cast<T*>(a.q_out) + (size_t)h0 * a.hd;
+        for (int j = 0; j < mine; ++j) {
+            const int r = row_of(j);
+            const Unit<N> u(place_of(j), a.rot, a.pairing, a.cos_t != nullptr);
+            const T* from = src + (size_t)(t_first + r) * a.ldq;
+            T* to = dst + (size_t)(t_first + r) * a.H * a.hd;
+            float x[Q_HEADS][2 * N];
+            Angles<N> t;
 #pragma unroll
-            for (int j = 0; j < KEEP; ++j) {
-                const int i = base + j * S, r = i / units;
-                if (i >= total) break;
-                const Unit<N> u(i - r * units, a.rot, a.pairing, a.cos_t != nullptr);
-                const T* p = src + (size_t)(t_first + r) * a.ldq;
-                load_group<T, N>(p + u.ia, x[j]);
-                load_group<T, N>(p + u.ib, x[j] + N);
+            for (int h = 0; h < Q_HEADS; ++h) {
+                if (h >= heads) break;
+                load_group<T, N>(from + h * a.hd + u.ia, x[h]);
+                load_group<T, N>(from + h * a.hd + u.ib, x[h] + N);
             }
+            t.load(a, u, first + r);
 #pragma unroll
-            for (int j = 0; j < KEEP; ++j) {
-                const int i = base + j * S, r = i / units;
-                if (i >= total) break;
-                const Unit<N> u(i - r * units, a.rot, a.pairing, a.cos_t != nullptr);
-                turn<N>(x[j], a, u, first + r);
-                T* p = dst + (size_t)r * a.H * a.hd;
-                store_group<T, N>(p + u.ia, x[j]);
-                store_group<T, N>(p + u.ib, x[j] + N);
+            for (int h = 0; h < Q_HEADS; ++h) {
+                if (h >= heads) break;
+                t.turn(x[h], a, u);
+                store_group<T, N>(to + h * a.hd + u.ia, x[h]);
+                store_group<T, N>(to + h * a.hd + u.ib, x[h] + N);
             }
         }
         return;
     }
-    const bool key = head < a.H + a.G;
-    const int g = key ? head - a.H : head - a.H - a.G;
+    const bool key = item < q_items + a.G;
+    const int g = item - q_items - (key ? 0 : a.G);
     if (page_no >= a.max_pages) return;
     const int page = PLM_PAGE_NO(a.block_table[(size_t)b * a.max_pages + page_no]);
     if (page <= 0) return;
@@ -144,25 +163,27 @@ kv8_append_kernel(const Append a) {
     const int place = first % PLM_PAGE;                          // rows before it are there already
     const int e_old = place ? kv8_exponent_of_scale(*scale_at) : KV8_E_MIN;
 
-    auto read = [&](int i, float* x) {
-        const int r = i / units;
-        const Unit<N> u(i - r * units, a.rot, a.pairing, rotate);
+    auto read = [&](int j, float* x) {
+        const int r = row_of(j);
+        const Unit<N> u(place_of(j), a.rot, a.pairing, rotate);
         const T* p = src + (size_t)(t_first + r) * ld;
         load_group<T, N>(p + u.ia, x);
         load_group<T, N>(p + u.ib, x + N);
-        turn<N>(x, a, u, first + r);
+        Angles<N> t;
+        t.load(a, u, first + r);
+        t.turn(x, a, u);
     };
     float x[KEEP][2 * N], most = 0.f;
 #pragma unroll
     for (int j = 0; j < KEEP; ++j) {
-        if (tid + j * S >= total) break;
-        read(tid + j * S, x[j]);
+        if (j >= mine) break;
+        read(j, x[j]);
 #pragma unroll
         for (int i = 0; i < 2 * N; ++i) most = fmaxf(most, kv8_magnitude(x[j][i]));
     }
-    for (int i = tid + KEEP * S; i < total; i += S) {
+    for (int j = KEEP; j < mine; ++j) {
         float y[2 * N];
-        read(i, y);
+        read(j, y);
 #pragma unroll
         for (int k = 0; k < 2 * N; ++k) most = fmaxf(most, kv8_magnitude(y[k]));
     }
@@ -189,17 +210,23 @@ kv8_append_kernel(const Append a) {
         }
     }
     const float up = kv8_pow2(-e);
-    auto put = [&](int i, const float* y) {
-        const int r = i / units;
-        const Unit<N> u(i - r * units, a.rot, a.pairing, rotate);
+    auto put = [&](int j, const float* y) {
+        const int r = row_of(j);
+        const Unit<N> u(place_of(j), a.rot, a.pairing, rotate);
         uint8_t* p = held + (size_t)(place + r) * a.hd;
-        if constexpr (N == 4) {
+        if constexpr (N >= 4) {
 #pragma unroll
             for (int half = 0; half < 2; ++half) {
-                const float* z = y + half * N;
-                *reinterpret_cast<uint32_t*>(p + (half ? u.ib : u.ia)) =
-                    kv8_pack(kv8_finite_or_nan(z[0]) * up, kv8_finite_or_nan(z[1]) * up) |
-                    kv8_pack(kv8_finite_or_nan(z[2]) * up, kv8_finite_or_nan(z[3]) * up) << 16;
+                uint32_t w[N / 4];
+#pragma unroll
+                for (int i = 0; i < N / 4; ++i) {
+                    const float* z = y + half * N + 4 * i;
+                    w[i] = kv8_pack(kv8_finite_or_nan(z[0]) * up, kv8_finite_or_nan(z[1]) * up) |
+                           kv8_pack(kv8_finite_or_nan(z[2]) * up, kv8_finite_or_nan(z[3]) * up) << 16;
+                }
+                uint8_t* to = p + (half ? u.ib : u.ia);
+                if constexpr (N == 8) *reinterpret_cast<uint2*>(to) = make_uint2(w[0], w[N / 4 - 1]);
+                else *reinterpret_cast<uint32_t*>(to) = w[0];
             }
         } else {
             const uint32_t two = kv8_pack(kv8_finite_or_nan(y[0]) * up, kv8_finite_or_nan(y[1]) * up);
@@ -209,24 +236,32 @@ kv8_append_kernel(const Append a) {
     };
 #pragma unroll
     for (int j = 0; j < KEEP; ++j) {
-        if (tid + j * S >= total) break;
-        put(tid + j * S, x[j]);
+        if (j >= mine) break;
+        put(j, x[j]);
     }
-    for (int i = tid + KEEP * S; i < total; i += S) {
+    for (int j = KEEP; j < mine; ++j) {
         float y[2 * N];
-        read(i, y);
-        put(i, y);
+        read(j, y);
+        put(j, y);
     }
     if (tid == 0) *scale_at = kv8_pow2(e);
 }
 
+template <typename T, int N, bool EVEN>
+int append(const Append& a, int n_seqs, int max_new, cudaStream_t stream) {
+    const int pages = 1 + (max_new + 62) / PLM_PAGE, items = (a.H + Q_HEADS - 1) / Q_HEADS + 2 * a.G;
+    // a warp takes an item of few rows as fast as more do, and four times as many items are in flight on an SM
+    if (max_new <= 4)
+        return plm_status_of(launch_pdl(kv8_append_kernel<T, N, 1, EVEN>, dim3(pages, (items + 3) / 4, n_seqs), dim3(128), 0, stream, a));
+    // four warps where a thread then keeps all it reads
+    if (PLM_PAGE * a.hd / (2 * N) <= 128 * (int)Held<N>::UNITS)
+        return plm_status_of(launch_pdl(kv8_append_kernel<T, N, 4, EVEN>, dim3(pages, items, n_seqs), dim3(128), 0, stream, a));
+    return plm_status_of(launch_pdl(kv8_append_kernel<T, N, 8, EVEN>, dim3(pages, items, n_seqs), dim3(256), 0, stream, a));
+}
 template <typename T, int N>
 int append(const Append& a, int n_seqs, int max_new, cudaStream_t stream) {
-    const int pages = 1 + (max_new + 62) / PLM_PAGE, heads = a.H + 2 * a.G;
-    // a warp takes an item of few rows as fast as eight do, and four times as many items are in flight on an SM
-    if (max_new <= 4)
-        return plm_status_of(launch_pdl(kv8_append_kernel<T, N, 1>, dim3(pages, (heads + 3) / 4, n_seqs), dim3(128), 0, stream, a));
-    return plm_status_of(launch_pdl(kv8_append_kernel<T, N, 8>, dim3(pages, heads, n_seqs), dim3(256), 0, stream, a));
+    const int units = a.hd / (2 * N);
+    return (units & (units - 1)) == 0 && units <= 32 ? append<T, N, true>(a, n_seqs, max_new, stream) : append<T, N, false>(a, n_seqs, max_new, stream);
 }
 
 // ------------------------------------------------------------------------------------------------ attention, fp32
@@ -235,6 +270,8 @@ int append(const Append& a, int n_seqs, int max_new, cudaStream_t stream) {
 // a key for the scores, a lane VEC components for the sums; running maximum and sum a row.  The ranges' partial results
 // (sum, maximum, denominator) meet in kv8_merge_kernel.
 constexpr int WARPS = 4;
+
+template <bool V> struct Const { static constexpr bool value = V; };
 
 template <typename T, int RPW, int VEC>
 __global__ void __launch_bounds__(WARPS * 32)
@@ -250,10 +287,12 @@ kv8_rows_kernel(const T* q, const uint8_t* kc, const uint8_t* vc, const float* k
     pdl_wait();
     pdl_launch_dependents();
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, R = H / G;
-    const int g = blockIdx.y / n_splits, split = blockIdx.y - g * n_splits;
+    // CTAs start in the order of their index: the tiles that see most keys first, of all kv heads
+    const unsigned lin = blockIdx.y * gridDim.x + blockIdx.x;
+    const int which = lin % gridDim.y, g = which / n_splits, split = which - g * n_splits;
     const Kv8Seq sq = kv8_seq(step, blockIdx.z);
-    const long pair0 = (long)blockIdx.x * ROWS, n_pairs = (long)sq.n_new * R;
-    if (pair0 >= n_pairs) return;
+    const long n_pairs = (long)sq.n_new * R, pair0 = ((n_pairs + ROWS - 1) / ROWS - 1 - (long)(lin / gridDim.y)) * ROWS;
+    if (pair0 < 0) return;
     const int pos_first = sq.pos0 + (int)(pair0 / R), pos_last = sq.pos0 + (int)(min(pair0 + ROWS, n_pairs) - 1) / R;
     // the walk: kept first positions that lie before the window's first group of 32, then the window's
     const int lo0 = plm_first_key(pos_first, window), g_lo = lo0 / 32;
@@ -288,6 +327,7 @@ kv8_rows_kernel(const T* q, const uint8_t* kc, const uint8_t* vc, const float* k
         const size_t base = (((size_t)page * G + g) * PLM_PAGE + key0 % PLM_PAGE) * hd;
         const float sk = ksc[(size_t)page * G + g], sv = vsc[(size_t)page * G + g];
         __syncthreads();                                             // what was there has been read (and q is there)
+        bool nan = false;
         for (int i = threadIdx.x; i < 32 * quads; i += WARPS * 32) {
             const int j = i / quads, c = i % quads * 4;
             float4 kv = make_float4(0.f, 0.f, 0.f, 0.f), vv = kv;
@@ -298,16 +338,17 @@ kv8_rows_kernel(const T* q, const uint8_t* kc, const uint8_t* vc, const float* k
                 const float2 v0 = kv8_floats(vw & 0xffffu), v1 = kv8_floats(vw >> 16);
                 kv = make_float4(k0.x * sk, k0.y * sk, k1.x * sk, k1.y * sk);
                 vv = make_float4(v0.x * sv, v0.y * sv, v1.x * sv, v1.y * sv);
+                nan |= !(v0.x == v0.x && v0.y == v0.y && v1.x == v1.x && v1.y == v1.y);
             }
             *reinterpret_cast<float4*>(ks + j * (hd + 4) + c) = kv;
             *reinterpret_cast<float4*>(vs + j * WIDE + c) = vv;
         }
-        __syncthreads();
+        nan = __syncthreads_or(nan);
         float dot[RPW];
 #pragma unroll
         for (int r = 0; r < RPW; ++r) dot[r] = 0.f;
         const float* kr = ks + lane * (hd + 4);
-#pragma unroll 2
+#pragma unroll 4
         for (int c = 0; c < hd; c += 4) {
             const float4 k4 = *reinterpret_cast<const float4*>(kr + c);
 #pragma unroll
@@ -330,22 +371,32 @@ kv8_rows_kernel(const T* q, const uint8_t* kc, const uint8_t* vc, const float* k
             ps[(r * WARPS + warp) * 32 + lane] = p;
         }
         __syncwarp();
-        for (int j = 0; j < 32; ++j) {
-            float v[VEC];
+        // NAN: a masked key's value may be NaN; it is not looked at (0 * NaN)
+        auto add = [&](auto skips) {
+#pragma unroll 2
+            for (int j0 = 0; j0 < 32; j0 += 4) {
+                float4 p4[RPW];
 #pragma unroll
-            for (int i = 0; i < VEC; i += VEC < 4 ? 2 : 4) {
-                if constexpr (VEC < 4) *reinterpret_cast<float2*>(v + i) = *reinterpret_cast<const float2*>(vs + j * WIDE + lane * VEC + i);
-                else *reinterpret_cast<float4*>(v + i) = *reinterpret_cast<const float4*>(vs + j * WIDE + lane * VEC + i);
-            }
+                for (int r = 0; r < RPW; ++r) p4[r] = *reinterpret_cast<const float4*>(ps + (r * WARPS + warp) * 32 + j0);
 #pragma unroll
-            for (int r = 0; r < RPW; ++r) {
-                const float p = ps[(r * WARPS + warp) * 32 + j];
-                if (p != 0.f) {                                      // (a masked key's value may be NaN: it is not looked at)
+                for (int k = 0; k < 4; ++k) {
+                    float v[VEC];
 #pragma unroll
-                    for (int i = 0; i < VEC; ++i) acc[r][i] = fmaf(p, v[i], acc[r][i]);
+                    for (int i = 0; i < VEC; i += VEC < 4 ? 2 : 4) {
+                        if constexpr (VEC < 4) *reinterpret_cast<float2*>(v + i) = *reinterpret_cast<const float2*>(vs + (j0 + k) * WIDE + lane * VEC + i);
+                        else *reinterpret_cast<float4*>(v + i) = *reinterpret_cast<const float4*>(vs + (j0 + k) * WIDE + lane * VEC + i);
+                    }
+#pragma unroll
+                    for (int r = 0; r < RPW; ++r) {
+                        const float p = k == 0 ? p4[r].x : k == 1 ? p4[r].y : k == 2 ? p4[r].z : p4[r].w;
+#pragma unroll
+                        for (int i = 0; i < VEC; ++i) acc[r][i] = fmaf(p, decltype(skips)::value && p == 0.f ? 0.f : v[i], acc[r][i]);
+                    }
                 }
             }
-        }
+        };
+        if (nan) add(Const<true>());
+        else add(Const<false>());
     }
 #pragma unroll
     for (int r = 0; r < RPW; ++r) {
@@ -446,12 +497,16 @@ extern "C" int plm_kv8_append(const void* q_in, const void* k_in, const void* v_
     if (((uintptr_t)kc | (uintptr_t)vc) & 15) return PLM_ERR_ALIGN;
     const Append a = {q_in, k_in, v_in, q_out, (uint8_t*)kc, (uint8_t*)vc, ks, vs, cos_t, sin_t, seq_start, seq_kv_len, block_table,
                       ldq, ldk, ldv, max_pages, n_table, H, G, hd, rot, pairing};
-    // groups of four where every group of the rows lies on a boundary of its own size
-    const uintptr_t rows = (uintptr_t)q_in | (uintptr_t)k_in | (uintptr_t)v_in | (uintptr_t)q_out;
-    const bool four = (!cos_t || (rot % 8 == 0 && !(((uintptr_t)cos_t | (uintptr_t)sin_t) & 15))) && !(rows & (dtype == PLM_F32 ? 15 : 7)) &&
-                      !((ldq | ldk | ldv) & 3);
-    if (dtype == PLM_F32) return four ? append<float, 4>(a, n_seqs, max_new, stream) : append<float, 1>(a, n_seqs, max_new, stream);
-    if (dtype == PLM_BF16) return four ? append<bf16, 4>(a, n_seqs, max_new, stream) : append<bf16, 1>(a, n_seqs, max_new, stream);
+    // N numbers at a time where all of them lie on a boundary of their own size, in the rows, the tables and the cache
+    const uintptr_t rows = (uintptr_t)q_in | (uintptr_t)k_in | (uintptr_t)v_in | (uintptr_t)q_out, tables = (uintptr_t)cos_t | (uintptr_t)sin_t;
+    const int item = dtype == PLM_F32 ? 4 : 2;
+    auto fits = [&](int n) {
+        return hd % (2 * n) == 0 && (!cos_t || (rot % (2 * n) == 0 && !(tables & 15))) && !(rows & (n * item - 1)) && !((ldq | ldk | ldv) & (n - 1));
+    };
+    if (dtype == PLM_F32) return fits(4) ? append<float, 4>(a, n_seqs, max_new, stream) : append<float, 1>(a, n_seqs, max_new, stream);
+    if (dtype == PLM_BF16)
+        return fits(8) ? append<bf16, 8>(a, n_seqs, max_new, stream)
+                       : fits(4) ? append<bf16, 4>(a, n_seqs, max_new, stream) : append<bf16, 1>(a, n_seqs, max_new, stream);
     return PLM_ERR_DTYPE;
 }
 

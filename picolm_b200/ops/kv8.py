@@ -17,7 +17,8 @@ from typing import Optional
 import torch
 
 from ..csrc.build import attention_variant
-from ._lib import PAGE_TOKENS, SM_COUNT, KernelError, _check, _dev, _dt, _fn, _i32, _p, _stream, set_bounds, status_word
+from ._lib import (CHECKED, PAGE_TOKENS, SM_COUNT, TRACED, KernelError, _check, _dev, _dt, _fn, _i32, _p, _stream, set_bounds,
+                   status_word)
 from .attention import _bias_check, _sink_check
 
 KV8_DTYPE = torch.float8_e4m3fn
@@ -29,26 +30,44 @@ def kv8_supported(head_dim: int) -> bool:
     return head_dim % 8 == 0 and 8 <= head_dim <= KV8_MAX_HEAD_DIM
 
 
-def _cache_check(what, k_cache, v_cache, k_scale, v_scale, G, hd, device):
+# The checks run on every launch of a decode step, so they are written to be quick: a tensor's device is one integer (-1: not on a
+# CUDA device), and what a message says is put together where it is raised.
+def _misplaced(what: str, dev: int, named) -> None:
+    """Raises for the first of the tensors that is not on device `dev` or not contiguous."""
+    for t, name in named:
+        _dev(t, name)
+        if t.get_device() != dev:
+            raise KernelError(f"{what}: the rows are on cuda:{dev}, {name} on {t.device}")
+
+
+def _current(dev: int) -> None:
+    if dev != torch.cuda.current_device():
+        raise KernelError(f"the tensors are on cuda:{dev}, the current device is cuda:{torch.cuda.current_device()}")
+
+
+def _cache_check(what, k_cache, v_cache, k_scale, v_scale, G, hd, dev):
+    if k_cache.get_device() != dev or v_cache.get_device() != dev or k_scale.get_device() != dev or v_scale.get_device() != dev or not (
+            k_cache.is_contiguous() and v_cache.is_contiguous() and k_scale.is_contiguous() and v_scale.is_contiguous()):
+        _misplaced(what, dev, ((k_cache, "k_cache"), (v_cache, "v_cache"), (k_scale, "k_scale"), (v_scale, "v_scale")))
     if not kv8_supported(hd):
         raise KernelError(f"{what}: head_dim {hd} is not supported (a multiple of 8 up to {KV8_MAX_HEAD_DIM})")
-    for c, s, n in ((k_cache, k_scale, "k"), (v_cache, v_scale, "v")):
-        _dev(c, n + "_cache"), _dev(s, n + "_scale")
-        if c.dtype != KV8_DTYPE or c.dim() != 4 or c.shape[1:] != (G, PAGE_TOKENS, hd):
-            raise KernelError(f"{what}: {n}_cache must be [pages, {G}, {PAGE_TOKENS}, {hd}] of {KV8_DTYPE}, got {c.dtype} {tuple(c.shape)}")
-        if s.dtype != torch.float32 or s.shape != c.shape[:2]:
-            raise KernelError(f"{what}: {n}_scale must be float32 [pages, {G}], got {s.dtype} {tuple(s.shape)}")
-        if c.device != device or s.device != device:
-            raise KernelError(f"{what}: the rows are on {device}, {n}_cache on {c.device}, {n}_scale on {s.device}")
-    if k_cache.shape != v_cache.shape:
-        raise KernelError(f"{what}: k_cache has {k_cache.shape[0]} pages, v_cache {v_cache.shape[0]}")
+    shape = k_cache.shape
+    if k_cache.dtype is not KV8_DTYPE or v_cache.dtype is not KV8_DTYPE or len(shape) != 4 or shape[1:] != (G, PAGE_TOKENS, hd) or v_cache.shape != shape:
+        raise KernelError(f"{what}: k_cache and v_cache must be [pages, {G}, {PAGE_TOKENS}, {hd}] of {KV8_DTYPE}, got {k_cache.dtype} {tuple(shape)} and "
+                          f"{v_cache.dtype} {tuple(v_cache.shape)}")
+    if k_scale.dtype is not torch.float32 or v_scale.dtype is not torch.float32 or k_scale.shape != shape[:2] or v_scale.shape != shape[:2]:
+        raise KernelError(f"{what}: k_scale and v_scale must be float32 [{shape[0]}, {G}], got {k_scale.dtype} {tuple(k_scale.shape)} and "
+                          f"{v_scale.dtype} {tuple(v_scale.shape)}")
 
 
-def _step_check(what, device, table, *ints):
-    for t, n in ints + ((table, "block_table"),):
-        _i32(t, n)
-        if t.device != device:
-            raise KernelError(f"{what}: the rows are on {device}, {n} on {t.device}")
+def _step_check(what, dev, table, first, second, names):
+    if first.get_device() != dev or second.get_device() != dev or table.get_device() != dev or first.dtype is not torch.int32 or \
+            second.dtype is not torch.int32 or table.dtype is not torch.int32 or not (first.is_contiguous() and second.is_contiguous() and
+                                                                                      table.is_contiguous()):
+        named = ((first, names[0]), (second, names[1]), (table, "block_table"))
+        _misplaced(what, dev, named)
+        for t, name in named:
+            _i32(t, name)
     if table.dim() != 2 or table.shape[1] == 0:
         raise KernelError(f"{what}: block_table must be [sequences, pages a sequence], got {tuple(table.shape)}")
 
@@ -63,46 +82,47 @@ def _sequences_check(what, seq_start, seq_kv_len, table, rows: int, max_new: int
     return B
 
 
-def _on(device) -> None:
-    if device.index is not None and device.index != torch.cuda.current_device():
-        raise KernelError(f"the tensors are on {device}, the current device is cuda:{torch.cuda.current_device()}")
-
-
-def _bounds(library, flags, k_cache, table, device, n_table: int = 0) -> None:
+def _bounds(library, flags, k_cache, table, n_table: int = 0) -> None:
     positions = table.shape[1] * PAGE_TOKENS
     set_bounds(library, flags, n_pages=k_cache.shape[0], n_seqs=table.shape[0],
-               n_positions=min(positions, n_table) if n_table else positions, device=device)
+               n_positions=min(positions, n_table) if n_table else positions, device=k_cache.device)
 
 
-def _append(what, q, k, v, q_out, k_cache, v_cache, k_scale, v_scale, cos, sin, seq_start, seq_kv_len, block_table, max_new,
-            H, G, hd, rotary_dim, pairing) -> None:
-    device, T = k.device, k.shape[0]
-    _on(device)
-    _cache_check(what, k_cache, v_cache, k_scale, v_scale, G, hd, device)
-    _step_check(what, device, block_table, (seq_start, "seq_start"), (seq_kv_len, "seq_kv_len"))
+def _launched(code: int, say, kernels: int = 1, nbytes: int = 0, flops: int = 0) -> None:
+    _check(code, say() if code or TRACED else "", kernels, nbytes, flops)
+
+
+def _append(what, dev, T, q_at, k_at, v_at, dtype, item, lds, q_out, k_cache, v_cache, k_scale, v_scale, cos, sin, seq_start, seq_kv_len,
+            block_table, max_new, H, G, hd, rotary_dim, pairing) -> None:
+    """`q_at`, `k_at`, `v_at`: addresses of the rows, `lds` elements apart."""
+    _cache_check(what, k_cache, v_cache, k_scale, v_scale, G, hd, dev)
+    _current(dev)
+    _step_check(what, dev, block_table, seq_start, seq_kv_len, ("seq_start", "seq_kv_len"))
     B = _sequences_check(what, seq_start, seq_kv_len, block_table, T, max_new)
-    if pairing not in ("half", "adjacent"):
+    if pairing != "half" and pairing != "adjacent":
         raise KernelError(f"{what}: unknown pairing {pairing!r}")
-    if (cos is None) != (sin is None):
-        raise KernelError(f"{what}: cos and sin come together")
-    if cos is not None:
-        _dev(cos, "cos"), _dev(sin, "sin")
+    n_table = 0
+    if cos is not None or sin is not None:
+        if cos is None or sin is None:
+            raise KernelError(f"{what}: cos and sin come together")
+        if cos.get_device() != dev or sin.get_device() != dev or not (cos.is_contiguous() and sin.is_contiguous()):
+            _misplaced(what, dev, ((cos, "cos"), (sin, "sin")))
         if not 0 < rotary_dim <= hd or rotary_dim % 2:
             raise KernelError(f"{what}: rotary_dim {rotary_dim} must be even, positive and at most head_dim {hd}")
-        if cos.dtype != torch.float32 or sin.dtype != torch.float32 or cos.dim() != 2 or cos.shape[0] == 0 or \
-                cos.shape[1] != rotary_dim // 2 or sin.shape != cos.shape:
+        shape = cos.shape
+        if cos.dtype is not torch.float32 or sin.dtype is not torch.float32 or len(shape) != 2 or shape[0] == 0 or shape[1] != rotary_dim // 2 or \
+                sin.shape != shape:
             raise KernelError(f"{what}: cos / sin tables must be float32 [positions, rotary_dim / 2]")
-        if cos.device != device or sin.device != device:
-            raise KernelError(f"{what}: the rows are on {device}, the tables on {cos.device} and {sin.device}")
+        n_table = shape[0]
     if T == 0:
         return
-    _bounds("kv8", (), k_cache, block_table, device, cos.shape[0] if cos is not None else 0)
-    item = k.element_size()
-    _check(_fn("kv8", "plm_kv8_append")(
-        _p(q), _p(k), _p(v), _dt(k, "rows"), 0 if q is None else q.stride(0), k.stride(0), v.stride(0), _p(q_out), _p(k_cache), _p(v_cache),
-        _p(k_scale), _p(v_scale), _p(cos), _p(sin), 0 if cos is None else cos.shape[0], _p(seq_start), _p(seq_kv_len), _p(block_table),
-        block_table.shape[1], B, int(max_new), H, G, hd, rotary_dim if cos is not None else 0, 0 if pairing == "half" else 1, _stream()),
-        f"{what} T={T} H={H} G={G} hd={hd}", nbytes=T * ((2 * H + 2 * G) * hd * item + 2 * G * hd))
+    if CHECKED:
+        _bounds("kv8", (), k_cache, block_table, n_table)
+    code = _fn("kv8", "plm_kv8_append")(
+        q_at, k_at, v_at, dtype, *lds, None if q_out is None else q_out.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), k_scale.data_ptr(),
+        v_scale.data_ptr(), _p(cos), _p(sin), n_table, seq_start.data_ptr(), seq_kv_len.data_ptr(), block_table.data_ptr(), block_table.shape[1], B,
+        max_new, H, G, hd, rotary_dim if n_table else 0, 0 if pairing == "half" else 1, _stream())
+    _launched(code, lambda: f"{what} T={T} H={H} G={G} hd={hd}", 1, T * ((2 * H + 2 * G) * hd * item + 2 * G * hd))
 
 
 def rope_store_kv8(qkv: torch.Tensor, q_out: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, k_scale: torch.Tensor,
@@ -114,26 +134,29 @@ def rope_store_kv8(qkv: torch.Tensor, q_out: torch.Tensor, k_cache: torch.Tensor
     seq_start[b + 1], at most `max_new`, and ends at position seq_kv_len[b] - 1; its pages are row b of `block_table`.  A token at the
     first place of a page begins it: whatever the page held is forgotten.  Rows of no sequence are left alone, and so are their
     rows of q_out.  No page may belong to two sequences."""
-    _dev(qkv, "qkv"), _dev(q_out, "q_out")
-    T, H, G, hd = qkv.shape[0], num_heads, num_kv_heads, head_dim
-    if H <= 0 or G <= 0 or qkv.dim() != 2 or qkv.shape[1] != (H + 2 * G) * hd or q_out.shape != (T, H, hd) or q_out.dtype != qkv.dtype:
+    dev, H, G, hd = qkv.get_device(), num_heads, num_kv_heads, head_dim
+    if dev < 0 or q_out.get_device() != dev or not (qkv.is_contiguous() and q_out.is_contiguous()):
+        _misplaced("rope_store_kv8", dev, ((qkv, "qkv"), (q_out, "q_out")))
+    shape, width = qkv.shape, (H + 2 * G) * hd
+    if H <= 0 or G <= 0 or len(shape) != 2 or shape[1] != width or q_out.shape != (shape[0], H, hd) or q_out.dtype is not qkv.dtype:
         raise KernelError("rope_store_kv8: qkv / q_out shapes do not match the head counts")
-    if q_out.device != qkv.device:
-        raise KernelError(f"rope_store_kv8: qkv is on {qkv.device}, q_out on {q_out.device}")
-    _append("rope_store_kv8", qkv, qkv[:, H * hd:], qkv[:, (H + G) * hd:], q_out, k_cache, v_cache, k_scale, v_scale, cos, sin,
-            seq_start, seq_kv_len, block_table, max_new, H, G, hd, rotary_dim, pairing)
+    item, at = qkv.element_size(), qkv.data_ptr()
+    _append("rope_store_kv8", dev, shape[0], at, at + H * hd * item, at + (H + G) * hd * item, _dt(qkv, "qkv"), item, (width, width, width), q_out,
+            k_cache, v_cache, k_scale, v_scale, cos, sin, seq_start, seq_kv_len, block_table, int(max_new), H, G, hd, rotary_dim, pairing)
 
 
 def store_kv8(k: torch.Tensor, v: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, k_scale: torch.Tensor,
               v_scale: torch.Tensor, seq_start: torch.Tensor, seq_kv_len: torch.Tensor, block_table: torch.Tensor,
               max_new: int) -> None:
     """Keys and values [T, G, hd] as they are (normed and rotated before) to the 8-bit cache; the rest as in `rope_store_kv8`."""
-    _dev(k, "k"), _dev(v, "v")
-    if k.dim() != 3 or v.shape != k.shape or v.dtype != k.dtype or v.device != k.device:
-        raise KernelError("store_kv8: k and v must be [T, G, head_dim] of one type on one device")
+    dev = k.get_device()
+    if dev < 0 or v.get_device() != dev or not (k.is_contiguous() and v.is_contiguous()):
+        _misplaced("store_kv8", dev, ((k, "k"), (v, "v")))
+    if k.dim() != 3 or v.shape != k.shape or v.dtype is not k.dtype:
+        raise KernelError("store_kv8: k and v must be [T, G, head_dim] of one type")
     T, G, hd = k.shape
-    _append("store_kv8", None, k, v, None, k_cache, v_cache, k_scale, v_scale, None, None, seq_start, seq_kv_len, block_table,
-            max_new, 0, G, hd, 0, "half")
+    _append("store_kv8", dev, T, None, k.data_ptr(), v.data_ptr(), _dt(k, "k"), k.element_size(), (0, G * hd, G * hd), None, k_cache, v_cache, k_scale,
+            v_scale, None, None, seq_start, seq_kv_len, block_table, int(max_new), 0, G, hd, 0, "half")
 
 
 # ------------------------------------------------------------------ attention
@@ -185,78 +208,93 @@ def kv8_streams(walks: int, rows: int, max_kv_len: int, head_dim: int) -> bool:
     return streamed < -(-walks // SM_COUNT) * pages
 
 
-def _attend(what, q, k_cache, v_cache, k_scale, v_scale, block_table, ints, max_new, max_kv_len, num_kv_heads, scale, window, out,
-            sink, keep_first, slopes, n_splits):
-    _dev(q, "q")
+_variants = {}
+
+
+def _variant(head_dim: int, family: str):
+    v = _variants.get((head_dim, family))
+    if v is None:
+        v = _variants[head_dim, family] = attention_variant(head_dim, family)
+    return v
+
+
+def _attend(what, q, k_cache, v_cache, k_scale, v_scale, block_table, first, second, decode, max_new, max_kv_len, num_kv_heads, scale,
+            window, out, sink, keep_first, slopes, n_splits):
+    dev, G = q.get_device(), num_kv_heads
+    if dev < 0 or not q.is_contiguous():
+        _dev(q, "q")
     if q.dim() != 3:
         raise KernelError(f"{what}: q must be [T, heads, head_dim], got {tuple(q.shape)}")
-    device = q.device
     T, H, hd = q.shape
-    G = num_kv_heads
-    _on(device)
     if G <= 0 or H % G:
         raise KernelError(f"{what}: the number of heads is not a multiple of the number of KV heads")
-    _dt(q, "q")
-    _cache_check(what, k_cache, v_cache, k_scale, v_scale, G, hd, device)
-    _sink_check(sink, H), _bias_check(keep_first, window, slopes, H)
-    for t, n in ((sink, "sink"), (slopes, "slopes")):
-        if t is not None and t.device != device:
-            raise KernelError(f"{what}: q is on {device}, {n} on {t.device}")
+    dtype = _dt(q, "q")
+    _cache_check(what, k_cache, v_cache, k_scale, v_scale, G, hd, dev)
+    _current(dev)
+    if sink is not None or slopes is not None or keep_first:
+        _sink_check(sink, H), _bias_check(keep_first, window, slopes, H)
+        for t, n in ((sink, "sink"), (slopes, "slopes")):
+            if t is not None and t.get_device() != dev:
+                raise KernelError(f"{what}: q is on {q.device}, {n} on {t.device}")
     if not scale > 0:
         raise KernelError(f"{what}: the scale must be positive, got {scale}")
     if n_splits is not None and not 0 <= n_splits <= KV8_CLUSTER_SPLITS:
         raise KernelError(f"{what}: n_splits must lie in 0 .. {KV8_CLUSTER_SPLITS}, got {n_splits}")
-    decode = ints[0][1] == "tok_pos"
-    _step_check(what, device, block_table, *ints)
     if decode:
-        if ints[0][0].shape != (T,) or ints[1][0].shape != (T,):
-            raise KernelError(f"{what}: tok_pos and tok_seq must be [{T}], got {tuple(ints[0][0].shape)} and {tuple(ints[1][0].shape)}")
+        _step_check(what, dev, block_table, first, second, ("tok_pos", "tok_seq"))
+        if first.shape != (T,) or second.shape != (T,):
+            raise KernelError(f"{what}: tok_pos and tok_seq must be [{T}], got {tuple(first.shape)} and {tuple(second.shape)}")
         B = T
     else:
-        B = _sequences_check(what, ints[0][0], ints[1][0], block_table, T, max_new)
+        _step_check(what, dev, block_table, first, second, ("seq_start", "seq_kv_len"))
+        B = _sequences_check(what, first, second, block_table, T, max_new)
     if out is None:
-        out = torch.empty((T, H * hd), dtype=q.dtype, device=device)
-    elif out.dtype != q.dtype or out.shape != (T, H * hd) or out.device != device or not out.is_contiguous():
-        raise KernelError(f"{what}: out must be a contiguous {q.dtype} [{T}, {H * hd}] tensor on {device}")
+        out = torch.empty((T, H * hd), dtype=q.dtype, device=q.device)
+    elif out.dtype is not q.dtype or out.shape != (T, H * hd) or out.get_device() != dev or not out.is_contiguous():
+        raise KernelError(f"{what}: out must be a contiguous {q.dtype} [{T}, {H * hd}] tensor on {q.device}")
     if T == 0 or B == 0:
         return out
-    step = (_p(ints[0][0]), _p(ints[1][0]), None, None) if decode else (None, None, _p(ints[0][0]), _p(ints[1][0]))
-    cache = (_p(k_cache), _p(v_cache), _p(k_scale), _p(v_scale))
-    tail = (float(scale), int(window or 0))
+    max_new, max_kv_len = int(max_new), max(1, int(max_kv_len))
+    step = (first.data_ptr(), second.data_ptr(), None, None) if decode else (None, None, first.data_ptr(), second.data_ptr())
+    cache = (k_cache.data_ptr(), v_cache.data_ptr(), k_scale.data_ptr(), v_scale.data_ptr(), out.data_ptr())
+    masks = (float(scale), int(window or 0))
     rest = (_p(sink), int(keep_first), _p(slopes), _stream())
     rows = max_new * (H // G)
     seen = max_kv_len if not window or window < 0 else min(max_kv_len, window + keep_first + max_new + 2 * PAGE_TOKENS)
-    need = dict(nbytes=B * seen * 2 * G * hd + 2 * T * H * hd * q.element_size(), flops=4 * T * H * hd * seen)
-    say = f"{what} T={T} H={H} G={G} hd={hd}"
+    table, pages = block_table.data_ptr(), block_table.shape[1]
+    need = (B * seen * 2 * G * hd + 2 * T * H * hd * q.element_size(), 4 * T * H * hd * seen) if TRACED else ()
     if not attention_kv8_mma_supported(q):
         ctas = B * G * (-(-rows // 32) if rows > 4 else 1)
-        splits = n_splits or max(1, min(4 * SM_COUNT // max(ctas, 1), seen // 64, 256, 65535 // G))
-        ws = torch.empty((T * H * splits * (hd + 2),), dtype=torch.float32, device=device) if splits > 1 else None
-        _bounds("kv8", (), k_cache, block_table, device)
-        _check(_fn("kv8", "plm_kv8_attention_rows")(
-            _p(q), _dt(q, "q"), *cache, _p(out), _p(ws), *step, _p(block_table), block_table.shape[1], T, B, int(max_new), H, G, hd, *tail,
-            splits, *rest), f"{say} rows splits={splits}", kernels=2 if ws is not None else 1, **need)
-        return out
-    lib, flags = attention_variant(hd, "attention_kv8")
-    _bounds(lib, flags, k_cache, block_table, device)
-    if decode or kv8_streams(B * G, rows, seen, hd):
+        splits = n_splits or max(1, min(4 * SM_COUNT // ctas, seen // 64, 256, 65535 // G))
+        ws = torch.empty((T * H * splits * (hd + 2),), dtype=torch.float32, device=q.device) if splits > 1 else None
+        if CHECKED:
+            _bounds("kv8", (), k_cache, block_table)
+        code = _fn("kv8", "plm_kv8_attention_rows")(q.data_ptr(), dtype, *cache, _p(ws), *step, table, pages, T, B, max_new, H, G, hd, *masks, splits, *rest)
+        _launched(code, lambda: f"{what} T={T} H={H} G={G} hd={hd} rows splits={splits}", 1 if ws is None else 2, *need)
+    elif decode or kv8_streams(B * G, rows, seen, hd):
+        lib, flags = _variant(hd, "attention_kv8")
+        if CHECKED:
+            _bounds(lib, flags, k_cache, block_table)
         tile, at_once, floats = kv8_few_plan(hd, rows)
         walks = B * G * -(-rows // tile)
         splits = kv8_cluster_splits(walks, at_once, seen) if n_splits is None else n_splits
-        ws = None if splits else torch.empty((at_once * floats + 2 * walks,), dtype=torch.float32, device=device)
-        _check(_fn(lib, "plm_kv8_attention_few", flags)(
-            _p(q), *cache, _p(out), _p(ws), *step, _p(block_table), block_table.shape[1], T, B, int(max_new), H, G, *tail, splits, at_once, *rest),
-            f"{say} few splits={splits}", kernels=1 if splits else 2, **need)
-        return out
-    if hd in (64, 128):
-        lib, flags = attention_variant(hd, "attention_kv8_tc")
-        _bounds(lib, flags, k_cache, block_table, device)
-        _check(_fn(lib, "plm_kv8_attention_tc", flags)(
-            _p(q), *cache, _p(out), *step[2:], _p(block_table), block_table.shape[1], B, int(max_new), H, G, *tail, _p(status_word(device)),
-            *rest), f"{say} tc", **need)
-        return out
-    _check(_fn(lib, "plm_kv8_attention_tiles", flags)(
-        _p(q), *cache, _p(out), *step[2:], _p(block_table), block_table.shape[1], B, int(max_new), H, G, *tail, *rest), f"{say} tiles", **need)
+        ws = None if splits else torch.empty((at_once * floats + 2 * walks,), dtype=torch.float32, device=q.device)
+        code = _fn(lib, "plm_kv8_attention_few", flags)(q.data_ptr(), *cache, _p(ws), *step, table, pages, T, B, max_new, H, G, *masks, splits, at_once,
+                                                        *rest)
+        _launched(code, lambda: f"{what} T={T} H={H} G={G} hd={hd} few splits={splits}", 1 if splits else 2, *need)
+    elif hd == 64 or hd == 128:
+        lib, flags = _variant(hd, "attention_kv8_tc")
+        if CHECKED:
+            _bounds(lib, flags, k_cache, block_table)
+        code = _fn(lib, "plm_kv8_attention_tc", flags)(q.data_ptr(), *cache, *step[2:], table, pages, B, max_new, H, G, *masks, status_word(q.device).data_ptr(),
+                                                       *rest)
+        _launched(code, lambda: f"{what} T={T} H={H} G={G} hd={hd} tc", 1, *need)
+    else:
+        lib, flags = _variant(hd, "attention_kv8")
+        if CHECKED:
+            _bounds(lib, flags, k_cache, block_table)
+        code = _fn(lib, "plm_kv8_attention_tiles", flags)(q.data_ptr(), *cache, *step[2:], table, pages, B, max_new, H, G, *masks, *rest)
+        _launched(code, lambda: f"{what} T={T} H={H} G={G} hd={hd} tiles", 1, *need)
     return out
 
 
@@ -268,8 +306,7 @@ def attention_kv8_decode(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.
     """Attention of single query tokens (one per row of q [T, H, hd], at position tok_pos[t] of sequence tok_seq[t]) over the 8-bit
     cache; returns [T, H * hd].  `max_kv_len`: an upper bound of tok_pos + 1, for the choice of how many ranges the keys are cut
     into (`n_splits` sets it: 1 to 8 ranges, or 0, all keys of the step dealt out over one wave of CTAs).  `window`, `sink`, `keep_first`, `slopes`: see `attention_rows`."""
-    return _attend("attention_kv8_decode", q, k_cache, v_cache, k_scale, v_scale, block_table, ((tok_pos, "tok_pos"), (tok_seq, "tok_seq")),
-                   1, max_kv_len, num_kv_heads, scale, window, out, sink, keep_first, slopes, n_splits)
+    return _attend("attention_kv8_decode", q, k_cache, v_cache, k_scale, v_scale, block_table, tok_pos, tok_seq, True, 1, max_kv_len, num_kv_heads, scale, window, out, sink, keep_first, slopes, n_splits)
 
 
 def attention_kv8_prefill(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, k_scale: torch.Tensor,
@@ -280,6 +317,5 @@ def attention_kv8_prefill(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch
     """Causal attention of every sequence's new tokens (rows seq_start[b] .. seq_start[b + 1] of q [T, H, hd], at most `max_new`) over
     its keys 0 .. seq_kv_len[b] - 1 (at most `max_kv_len`) in the 8-bit cache; returns [T, H * hd].  Rows of no sequence are left as they
     are in `out`.  The rest as in `attention_kv8_decode`."""
-    return _attend("attention_kv8_prefill", q, k_cache, v_cache, k_scale, v_scale, block_table,
-                   ((seq_start, "seq_start"), (seq_kv_len, "seq_kv_len")), max_new, max_kv_len, num_kv_heads, scale, window, out, sink,
+    return _attend("attention_kv8_prefill", q, k_cache, v_cache, k_scale, v_scale, block_table, seq_start, seq_kv_len, False, max_new, max_kv_len, num_kv_heads, scale, window, out, sink,
                    keep_first, slopes, n_splits)
