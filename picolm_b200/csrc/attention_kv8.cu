@@ -59,14 +59,6 @@ __device__ __forceinline__ uint32_t turned(uint32_t x) {      // an 8 x 8 matrix
     asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(x));
     return r;
 }
-__device__ __forceinline__ void ldsm_x4(uint32_t (&r)[4], uint32_t addr) {
-    asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0, %1, %2, %3}, [%4];"
-                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(addr) : "memory");
-}
-__device__ __forceinline__ void ldsm_x4_t(uint32_t (&r)[4], uint32_t addr) {
-    asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0, %1, %2, %3}, [%4];"
-                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(addr) : "memory");
-}
 // bytes that are NaN (e4m3: 0x7f and 0xff): 0x80 in their places
 __device__ __forceinline__ uint32_t nan_bytes(uint32_t w) { return ((w & 0x7f7f7f7fu) + 0x01010101u) & 0x80808080u; }
 __device__ __forceinline__ uint32_t without(uint32_t w, uint32_t marks) { return w & ~(marks | (marks - (marks >> 7))); }
@@ -211,7 +203,7 @@ template <int NG> struct Few {
 constexpr int MIN_UNITS = 4;                     // of a warp's range, so that its start and a partial result are worth it
 template <int COLS, int KB> struct Deal {
     const Kv8Step& step;
-    int n_seqs, G, R, window, keep;
+    int n_seqs, G, R, window, keep, most;         // (most: tiles of a sequence that the launch knows of)
     __device__ __forceinline__ void of(int b, int& units, int& tiles) const {
         const Kv8Seq q = kv8_seq(step, b);
         units = tiles = 0;
@@ -219,7 +211,7 @@ template <int COLS, int KB> struct Deal {
         const int last = q.pos0 + q.n_new - 1;
         const Walk w(q.pos0, last, window, keep);
         units = w.n_pages * (PLM_PAGE / KB) - (PLM_PAGE - 1 - last % PLM_PAGE) / KB;
-        tiles = (q.n_new * R + COLS - 1) / COLS;
+        tiles = min(most, (q.n_new * R + COLS - 1) / COLS);
     }
     __device__ __forceinline__ unsigned long long all(int b) const {
         int u, t;
@@ -584,7 +576,7 @@ kv8_stream_kernel(const bf16* q, const Cache cache, bf16* __restrict__ out, floa
         if (n8 == 0) *reinterpret_cast<float2*>(row + HD) = make_float2(m, l);
     };
 
-    const Deal<COLS, KB> deal = {step, n_seqs, G, R, window, keep};
+    const Deal<COLS, KB> deal = {step, n_seqs, G, R, window, keep, tiles};
     if constexpr (CLUSTER) {
         float* part = reinterpret_cast<float*>(sm_raw + Few<NG>::Q_BYTES);         // after the walk, in the rings' place: [WARPS][COLS][ROW]
         float* mine = part + WARPS * COLS * ROW;                                   // [COLS][ROW]
@@ -709,10 +701,10 @@ kv8_join_kernel(const float* ws, const int2* pieces, bf16* __restrict__ out, con
     pdl_launch_dependents();
     const int R = H / G, b = blockIdx.z, at = blockIdx.y * JOIN + threadIdx.x, row = at / HD, d = at - row * HD;
     const int g = blockIdx.x / tiles, tile = blockIdx.x - g * tiles, pair = tile * COLS + row;
-    const int t0 = step.tok_pos ? b : step.seq_start[b], n_new = step.tok_pos ? 1 : step.seq_start[b + 1] - t0;
-    if (tile * COLS >= n_new * R) return;                            // (no walk)
+    const Kv8Seq sq = kv8_seq(step, b);
+    if (tile * COLS >= sq.n_new * R) return;                         // (no walk)
     const int2 who = pieces[((size_t)b * G + g) * tiles + tile];
-    if (who.y == 1 || row >= COLS || pair >= n_new * R) return;      // one warp had it all, or no such row
+    if (who.y == 1 || row >= COLS || pair >= sq.n_new * R) return;      // one warp had it all, or no such row
     auto place = [&](int i) { return ws + ((size_t)((who.x + i) * 2 + (i == 0 ? 1 : 0)) * COLS + row) * ROW; };
     float m = -INFINITY, l = 0.f, acc = 0.f;
     for (int i0 = 0; i0 < who.y; i0 += AT_ONCE) {
@@ -740,7 +732,7 @@ kv8_join_kernel(const float* ws, const int2* pieces, bf16* __restrict__ out, con
         }
     }
     const int h = g * R + pair % R;
-    out[((size_t)(t0 + pair / R) * H + h) * HD + d] = __float2bfloat16_rn(acc * kv8_inverse(m, l, sink ? sink + h : nullptr));
+    out[((size_t)(sq.t0 + pair / R) * H + h) * HD + d] = __float2bfloat16_rn(acc * kv8_inverse(m, l, sink ? sink + h : nullptr));
 }
 
 // The same for walks that many warps shared (few sequences): a block a row, in strands of every (512 / LANES)-th warp, the strands in
@@ -762,7 +754,15 @@ kv8_join_many_kernel(const float* ws, const int2* pieces, bf16* __restrict__ out
     const int n = who.y;
     if (n == 1) return;                                              // one warp had it all
     auto place = [&](int i) { return ws + ((size_t)((who.x + i) * 2 + (i == 0 ? 1 : 0)) * COLS + blockIdx.y) * ROW; };
-    float m = -INFINITY;
+    // everything that a thread reads of the first pieces is asked for before anything is waited for
+    const int strand = threadIdx.x / LANES, d = threadIdx.x % LANES;
+    float ahead[AT_ONCE], m = -INFINITY, l_first = 0.f;
+#pragma unroll
+    for (int k = 0; k < AT_ONCE; ++k) {
+        const int i = strand + k * STRANDS;
+        ahead[k] = d < HD && i < n ? place(i)[d] : 0.f;
+    }
+    if ((int)threadIdx.x < n) l_first = place(threadIdx.x)[HD + 1];
     for (int i = threadIdx.x; i < n; i += THREADS) m = fmaxf(m, factor[i] = place(i)[HD]);
     m = warp_max(m);
     if (lane == 0) red[warp] = m;
@@ -773,16 +773,18 @@ kv8_join_many_kernel(const float* ws, const int2* pieces, bf16* __restrict__ out
     for (int i = threadIdx.x; i < n; i += THREADS) {
         const float f = factor[i] == -INFINITY ? 0.f : exp2f(factor[i] - m);
         factor[i] = f;
-        l = fmaf(f, place(i)[HD + 1], l);
+        l = fmaf(f, i == (int)threadIdx.x ? l_first : place(i)[HD + 1], l);
     }
     l = warp_sum(l);
     __syncthreads();
     if (lane == 0) red[warp] = l;
-    const int strand = threadIdx.x / LANES, d = threadIdx.x % LANES;
     float acc = 0.f;
     if (d < HD) {
+#pragma unroll
+        for (int k = 0; k < AT_ONCE; ++k)
+            if (strand + k * STRANDS < n) acc = fmaf(factor[strand + k * STRANDS], ahead[k], acc);
 #pragma unroll 8
-        for (int i = strand; i < n; i += STRANDS) acc = fmaf(factor[i], place(i)[d], acc);
+        for (int i = strand + AT_ONCE * STRANDS; i < n; i += STRANDS) acc = fmaf(factor[i], place(i)[d], acc);
     }
     sums[threadIdx.x] = acc;
     __syncthreads();
@@ -799,6 +801,14 @@ kv8_join_many_kernel(const float* ws, const int2* pieces, bf16* __restrict__ out
 
 // -------------------------------------------------------------------------------------------- prompts
 #if PLM_HD != 64 && PLM_HD != 128                // (those on tcgen05: attention_kv8_tc.cu)
+__device__ __forceinline__ void ldsm_x4(uint32_t (&r)[4], uint32_t addr) {
+    asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0, %1, %2, %3}, [%4];"
+                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(addr) : "memory");
+}
+__device__ __forceinline__ void ldsm_x4_t(uint32_t (&r)[4], uint32_t addr) {
+    asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0, %1, %2, %3}, [%4];"
+                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(addr) : "memory");
+}
 constexpr int LDS = HD + 8;                      // halves of a row in shared memory: ldmatrix without bank conflicts
 constexpr size_t TILE_SMEM = (size_t)3 * 64 * LDS * 2;
 
@@ -1040,6 +1050,9 @@ int stream(const bf16* q, const Cache& cache, bf16* out, void* ws, const Kv8Step
     if (!ws)
         return plm_status_of(launch_pdl_cluster(kv8_stream_kernel<NG, true>, dim3(n_splits, (unsigned)(tiles * G), n_seqs), dim3(NT), dim3(n_splits, 1, 1),
                                                 smem, s, q, cache, out, none, pieces, step, n_seqs, H, G, (int)tiles, scale * LOG2E, window, sink, keep, slopes));
+    // (no more CTAs than the step can have work for)
+    const long most = (tiles * G * n_seqs * ((long)step.max_pages * (PLM_PAGE / Few<NG>::KB)) + WARPS * MIN_UNITS - 1) / (WARPS * MIN_UNITS);
+    if (n_ctas > most) n_ctas = (int)most;
     float* part = reinterpret_cast<float*>(ws);
     pieces = reinterpret_cast<int2*>(part + (size_t)n_ctas * WARPS * 2 * 8 * NG * ROW);
     int rc = plm_status_of(launch_pdl(kv8_stream_kernel<NG, false>, dim3(n_ctas), dim3(NT), smem, s, q, cache, out, part, pieces, step, n_seqs, H, G,

@@ -49,6 +49,12 @@ static_assert(SMEM <= 227 * 1024, "shared memory");
 // Registers a thread: launched with 128; the softmax's two warpgroups take 168 each, the other two keep 88: 2 * 168 + 2 * 88 = 4 * 128.
 constexpr int SOFTMAX_REGS = 168, OTHER_REGS = 88;
 
+#ifdef PLM_TEST_STALL
+__device__ int plm_stall = 0;                     // a test build: the pages' barriers are told of more bytes than come
+constexpr uint32_t SPIN_LIMIT = 4 * WAIT_LIMIT;
+#else
+constexpr uint32_t SPIN_LIMIT = 1u << 26;
+#endif
 __device__ __forceinline__ bool mbar_test(uint32_t bar, uint32_t parity) {
     uint32_t ok;
     asm volatile(
@@ -60,7 +66,7 @@ __device__ __forceinline__ bool mbar_test(uint32_t bar, uint32_t parity) {
 }
 // the hand-over per page between the issuer and the softmax threads: polls without being parked
 __device__ __forceinline__ bool mbar_spin(uint32_t bar, uint32_t parity, int* status, int where) {
-    for (uint32_t i = 0; i < (1u << 26); ++i)
+    for (uint32_t i = 0; i < SPIN_LIMIT; ++i)
         if (mbar_test(bar, parity)) return true;
     if (status) atomicCAS(status, 0, where);
     return false;
@@ -549,7 +555,11 @@ kv8_tc_kernel(const bf16* q, const Cache cache, bf16* __restrict__ out, const Kv
                 const size_t at = ((size_t)PLM_PAGE_NO(sq.pages[page_at(i)]) * G + g) * RAW_BYTES;
                 if (*(volatile int*)&s_abort) break;
                 if (!mbar_wait(raw_empty + 8 * rs, ((i / RS) & 1) ^ 1, status, 73)) { s_abort = 1; break; }
+#ifdef PLM_TEST_STALL
+                mbar_expect_tx(raw_full + 8 * rs, 2 * RAW_BYTES + (plm_stall ? 64 : 0));
+#else
                 mbar_expect_tx(raw_full + 8 * rs, 2 * RAW_BYTES);
+#endif
                 bulk_load(raw + rs * 2 * RAW_BYTES, cache.k + at, RAW_BYTES, raw_full + 8 * rs);
                 bulk_load(raw + rs * 2 * RAW_BYTES + RAW_BYTES, cache.v + at, RAW_BYTES, raw_full + 8 * rs);
                 issued = i + 1;
@@ -588,3 +598,9 @@ extern "C" int plm_kv8_attention_tc(const void* q, const void* kc, const void* v
     return plm_status_of(launch_pdl(more ? kv8_tc_kernel<true> : kv8_tc_kernel<false>, grid, dim3(NT), SMEM, stream, (const bf16*)q, cache,
                                     (bf16*)out, step, H, G, scale * LOG2E, window, status, sink, keep, slopes));
 }
+
+#ifdef PLM_TEST_STALL
+extern "C" int plm_test_stall(int on, cudaStream_t stream) {
+    return (int)cudaMemcpyToSymbolAsync(plm_stall, &on, sizeof(on), 0, cudaMemcpyHostToDevice, stream);
+}
+#endif

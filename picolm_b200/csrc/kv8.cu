@@ -419,14 +419,15 @@ kv8_rows_kernel(const T* q, const uint8_t* kc, const uint8_t* vc, const float* k
 }
 
 // out[row] = sum_s w_s acc_s / sum_s w_s l_s with w_s = exp2(m_s - max m), ranges in their order; ws [rows, n_splits, hd + 2]:
-// acc, m, l.  A block a row, a thread a component (or several).
+// acc, m, l.  A block a row, a thread a component (or several); grid (tokens of a sequence * H, sequences).
 template <typename T>
 __global__ void __launch_bounds__(128)
-kv8_merge_kernel(const float* ws, T* __restrict__ out, int n_splits, int hd, int H, const float* sink, const int* seq_start, int n_seqs) {
+kv8_merge_kernel(const float* ws, T* __restrict__ out, const Kv8Step step, int n_splits, int hd, int H, const float* sink) {
     pdl_wait();
     pdl_launch_dependents();
-    const size_t row = blockIdx.x;
-    if (kv8_of_no_sequence((int)(row / H), seq_start, n_seqs)) return;
+    const Kv8Seq sq = kv8_seq(step, blockIdx.y);
+    if ((int)(blockIdx.x / H) >= sq.n_new) return;
+    const size_t row = (size_t)sq.t0 * H + blockIdx.x;
     const float* p = ws + row * n_splits * (hd + 2);
     float m = -INFINITY, l = 0.f;
     for (int s = 0; s < n_splits; ++s) m = fmaxf(m, p[(size_t)s * (hd + 2) + hd]);
@@ -462,14 +463,14 @@ int rows_launch(dim3 grid, const void* q, const void* kc, const void* vc, const 
 
 template <typename T>
 int rows_any(const void* q, const void* kc, const void* vc, const float* ks, const float* vs, void* out, float* ws,
-             const Kv8Step& step, int n_rows, int n_seqs, int max_new, int H, int G, int hd, float scale, int window, int n_splits,
+             const Kv8Step& step, int n_seqs, int max_new, int H, int G, int hd, float scale, int window, int n_splits,
              const float* sink, int keep, const float* slopes, cudaStream_t stream) {
     const int R = H / G;
     const long pairs = (long)max_new * R;
     // few rows: one a warp, so that the CTAs are many; else eight, so that what is brought to shared memory is used often
     const bool few = pairs <= WARPS;
     const long tiles = few ? 1 : (pairs + 8 * WARPS - 1) / (8 * WARPS);
-    if (tiles > 0x7fffffffL || (long)G * n_splits > 65535 || n_seqs > 65535) return PLM_ERR_SHAPE;
+    if (tiles > 0x7fffffffL || (long)max_new * H > 0x7fffffffL || (long)G * n_splits > 65535 || n_seqs > 65535) return PLM_ERR_SHAPE;
     const dim3 grid((unsigned)tiles, G * n_splits, n_seqs);
     int rc;
 #define KV8_ROWS(RPW_, VEC_) rc = rows_launch<T, RPW_, VEC_>(grid, q, kc, vc, ks, vs, out, ws, step, H, G, hd, scale, window, n_splits, sink, keep, slopes, stream)
@@ -478,8 +479,8 @@ int rows_any(const void* q, const void* kc, const void* vc, const float* ks, con
     else { if (few) KV8_ROWS(1, 8); else KV8_ROWS(8, 8); }
 #undef KV8_ROWS
     if (rc != PLM_OK || n_splits == 1) return rc;
-    return plm_status_of(launch_pdl(kv8_merge_kernel<T>, dim3((unsigned)((long)n_rows * H)), dim3(128), 0, stream, (const float*)ws,
-                                    (T*)out, n_splits, hd, H, sink, step.seq_start, n_seqs));
+    return plm_status_of(launch_pdl(kv8_merge_kernel<T>, dim3((unsigned)((long)max_new * H), n_seqs), dim3(128), 0, stream, (const float*)ws,
+                                    (T*)out, step, n_splits, hd, H, sink));
 }
 
 }  // namespace
@@ -523,8 +524,8 @@ extern "C" int plm_kv8_attention_rows(const void* q, int dtype, const void* kc, 
     if ((uintptr_t)q & 15) return PLM_ERR_ALIGN;
     const Kv8Step step = {tok_pos, tok_seq, seq_start, seq_kv_len, block_table, max_pages};
     if (dtype == PLM_F32)
-        return rows_any<float>(q, kc, vc, ks, vs, out, ws, step, n_rows, n_seqs, max_new, H, G, hd, scale, window, n_splits, sink, keep, slopes, stream);
+        return rows_any<float>(q, kc, vc, ks, vs, out, ws, step, n_seqs, max_new, H, G, hd, scale, window, n_splits, sink, keep, slopes, stream);
     if (dtype == PLM_BF16)
-        return rows_any<bf16>(q, kc, vc, ks, vs, out, ws, step, n_rows, n_seqs, max_new, H, G, hd, scale, window, n_splits, sink, keep, slopes, stream);
+        return rows_any<bf16>(q, kc, vc, ks, vs, out, ws, step, n_seqs, max_new, H, G, hd, scale, window, n_splits, sink, keep, slopes, stream);
     return PLM_ERR_DTYPE;
 }

@@ -51,7 +51,8 @@ __device__ __forceinline__ int kv8_exponent_of_scale(float s) { return (int)(__f
 
 // A step's sequence as attention sees it.  With tok_pos every row of q is a token of its own (`b` is its number), at
 // position tok_pos[b] of the sequence whose pages are row tok_seq[b] of the table; otherwise `b` is a sequence of the step,
-// its new tokens are rows seq_start[b] .. seq_start[b + 1] and its keys 0 .. seq_kv_len[b] - 1.
+// its new tokens are rows seq_start[b] .. seq_start[b + 1] and its keys 0 .. seq_kv_len[b] - 1.  One whose positions its row of the table
+// does not hold counts as one without rows: nothing is read or written for it.
 struct Kv8Step {
     const int *tok_pos, *tok_seq, *seq_start, *seq_kv_len, *block_table;
     int max_pages;
@@ -73,12 +74,8 @@ __device__ __forceinline__ Kv8Seq kv8_seq(const Kv8Step& s, int b) {
         q.pos0 = q.n_new > 0 ? PLM_POSITION(s.seq_kv_len[b] - 1) + 1 - q.n_new : 0;
         q.pages = s.block_table + (size_t)b * s.max_pages;
     }
+    if (q.n_new < 0 || q.pos0 < 0 || q.pos0 > s.max_pages * PLM_PAGE - q.n_new) q.n_new = 0;
     return q;
-}
-
-// A row of q in front of the first sequence's or behind the last one's: no kernel looks at it or writes its result.
-__device__ __forceinline__ bool kv8_of_no_sequence(int row, const int* seq_start, int n_seqs) {
-    return seq_start && (row < seq_start[0] || row >= seq_start[n_seqs]);
 }
 
 // With a sink (one more term exp(sink) in the denominator) the factor that turns a row's sum_j exp2(s_j - m) v_j into its
