@@ -573,7 +573,7 @@ kv8_stream_kernel(const bf16* q, const Cache cache, bf16* __restrict__ out, floa
     auto put = [&](float* row, const float (&o)[MT][4], int e, float m, float l) {
 #pragma unroll
         for (int t = 0; t < MT; ++t) *reinterpret_cast<float2*>(row + value_component(t, n8)) = make_float2(o[t][e], o[t][2 + e]);
-        if (n8 == 0) *reinterpret_cast<float2*>(row + HD) = make_float2(m, l);
+        if (n8 == 0) *reinterpret_cast<float2*>(row + HD) = make_float2(kv8_top(m, l), l);
     };
 
     const Deal<COLS, KB> deal = {step, n_seqs, G, R, window, keep, tiles};

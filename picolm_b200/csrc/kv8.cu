@@ -111,6 +111,7 @@ kv8_append_kernel(const Append a) {
     const int t0 = a.seq_start[b], n_new = a.seq_start[b + 1] - t0;
     if (n_new <= 0) return;
     const int pos0 = PLM_POSITION(a.seq_kv_len[b] - 1) + 1 - n_new;
+    if (pos0 < 0) return;                                        // more tokens than the sequence is long
     const int page_no = pos0 / PLM_PAGE + blockIdx.x;
     const int first = max(pos0, page_no * PLM_PAGE), rows = min(pos0 + n_new, (page_no + 1) * PLM_PAGE) - first;
     if (rows <= 0) return;
@@ -244,6 +245,7 @@ kv8_append_kernel(const Append a) {
         read(j, y);
         put(j, y);
     }
+    if (W == 1) __syncwarp();                                    // (all have read the scale; more warps met at the maximum)
     if (tid == 0) *scale_at = kv8_pow2(e);
 }
 
@@ -412,7 +414,7 @@ kv8_rows_kernel(const T* q, const uint8_t* kc, const uint8_t* vc, const float* k
             else out[row * hd + d] = from_f32<T>(acc[r][i] * inv);
         }
         if (n_splits > 1 && lane == 0) {
-            ws[(row * n_splits + split) * (hd + 2) + hd] = m[r];
+            ws[(row * n_splits + split) * (hd + 2) + hd] = kv8_top(m[r], l[r]);
             ws[(row * n_splits + split) * (hd + 2) + hd + 1] = l[r];
         }
     }

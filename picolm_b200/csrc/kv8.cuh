@@ -78,10 +78,15 @@ __device__ __forceinline__ Kv8Seq kv8_seq(const Kv8Step& s, int b) {
     return q;
 }
 
+// The maximum that a partial result goes by where several are put together: ones with -inf are skipped as empty, and a NaN among the scores,
+// which is in l and not in the maximum, must not be.
+__device__ __forceinline__ float kv8_top(float m, float l) { return l == l ? m : fmaxf(m, 0.f); }
+
 // With a sink (one more term exp(sink) in the denominator) the factor that turns a row's sum_j exp2(s_j - m) v_j into its
-// result: 1 / (l + exp2(sink log2e - m)), written so that a sink far above the scores does not overflow.
+// result: 1 / (l + exp2(sink log2e - m)), written so that a sink far above the scores does not overflow.  A row sees its own key at least: with
+// m still -inf all its scores are -inf (a softmax of nothing, unless a sink is there) or NaN (then l is).
 __device__ __forceinline__ float kv8_inverse(float m, float l, const float* sink) {
-    if (m == -INFINITY) return 0.f;
+    if (m == -INFINITY) return sink && *sink > -INFINITY ? l : __int_as_float(0x7fffffff);
     if (!sink) return 1.f / l;
     const float sk = *sink * 1.4426950408889634f;
     if (sk <= m) return 1.f / (l + exp2f(sk - m));

@@ -116,6 +116,7 @@ def _append(what, dev, T, q_at, k_at, v_at, dtype, item, lds, q_out, k_cache, v_
         n_table = shape[0]
     if T == 0:
         return
+    max_new = min(max_new, T)
     if CHECKED:
         _bounds("kv8", (), k_cache, block_table, n_table)
     code = _fn("kv8", "plm_kv8_append")(
@@ -131,9 +132,10 @@ def rope_store_kv8(qkv: torch.Tensor, q_out: torch.Tensor, k_cache: torch.Tensor
                    head_dim: int, rotary_dim: int, pairing: str) -> None:
     """Rotate the query and key heads of `qkv` [T, (H + 2G) * hd] by their tokens' positions (cos / sin None: no rotation);
     write queries to `q_out` [T, H, hd], keys and values to the 8-bit cache.  Sequence b brings rows seq_start[b] ..
-    seq_start[b + 1], at most `max_new`, and ends at position seq_kv_len[b] - 1; its pages are row b of `block_table`.  A token at the
-    first place of a page begins it: whatever the page held is forgotten.  Rows of no sequence are left alone, and so are their
-    rows of q_out.  No page may belong to two sequences."""
+    seq_start[b + 1], at most `max_new`, and ends at position seq_kv_len[b] - 1; its pages are row b of `block_table`
+    (what lies behind that row's last page is not kept).  A token at the first place of a page begins it: whatever the page held is
+    forgotten.  One at an earlier place than the last follows what lies before it, and the page's scale stays at least as large as it
+    was.  Rows of no sequence are left alone, and so are their rows of q_out.  No page may belong to two sequences."""
     dev, H, G, hd = qkv.get_device(), num_heads, num_kv_heads, head_dim
     if dev < 0 or q_out.get_device() != dev or not (qkv.is_contiguous() and q_out.is_contiguous()):
         _misplaced("rope_store_kv8", dev, ((qkv, "qkv"), (q_out, "q_out")))
@@ -249,19 +251,22 @@ def _attend(what, q, k_cache, v_cache, k_scale, v_scale, block_table, first, sec
         _step_check(what, dev, block_table, first, second, ("seq_start", "seq_kv_len"))
         B = _sequences_check(what, first, second, block_table, T, max_new)
     if out is None:
-        out = torch.empty((T, H * hd), dtype=q.dtype, device=q.device)
+        out = q.new_empty((T, H * hd))
     elif out.dtype is not q.dtype or out.shape != (T, H * hd) or out.get_device() != dev or not out.is_contiguous():
         raise KernelError(f"{what}: out must be a contiguous {q.dtype} [{T}, {H * hd}] tensor on {q.device}")
     if T == 0 or B == 0:
         return out
-    max_new, max_kv_len = int(max_new), max(1, int(max_kv_len))
+    # (no sequence brings more than all rows, none is longer than its row of the table)
+    table, pages = block_table.data_ptr(), block_table.shape[1]
+    held = pages * PAGE_TOKENS
+    max_new, max_kv_len, keep_first = min(int(max_new), T), max(1, min(int(max_kv_len), held)), min(int(keep_first), held)
+    window = max(-held, min(int(window), held)) if window else 0
     step = (first.data_ptr(), second.data_ptr(), None, None) if decode else (None, None, first.data_ptr(), second.data_ptr())
     cache = (k_cache.data_ptr(), v_cache.data_ptr(), k_scale.data_ptr(), v_scale.data_ptr(), out.data_ptr())
-    masks = (float(scale), int(window or 0))
-    rest = (_p(sink), int(keep_first), _p(slopes), _stream())
+    masks = (float(scale), window)
+    rest = (_p(sink), keep_first, _p(slopes), _stream())
     rows = max_new * (H // G)
-    seen = max_kv_len if not window or window < 0 else min(max_kv_len, window + keep_first + max_new + 2 * PAGE_TOKENS)
-    table, pages = block_table.data_ptr(), block_table.shape[1]
+    seen = max_kv_len if window <= 0 else min(max_kv_len, window + keep_first + max_new + 2 * PAGE_TOKENS)
     need = (B * seen * 2 * G * hd + 2 * T * H * hd * q.element_size(), 4 * T * H * hd * seen) if TRACED else ()
     if not attention_kv8_mma_supported(q):
         ctas = B * G * (-(-rows // 32) if rows > 4 else 1)
@@ -305,8 +310,11 @@ def attention_kv8_decode(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.
                          slopes: Optional[torch.Tensor] = None, n_splits: Optional[int] = None) -> torch.Tensor:
     """Attention of single query tokens (one per row of q [T, H, hd], at position tok_pos[t] of sequence tok_seq[t]) over the 8-bit
     cache; returns [T, H * hd].  `max_kv_len`: an upper bound of tok_pos + 1, for the choice of how many ranges the keys are cut
-    into (`n_splits` sets it: 1 to 8 ranges, or 0, all keys of the step dealt out over one wave of CTAs).  `window`, `sink`, `keep_first`, `slopes`: see `attention_rows`."""
-    return _attend("attention_kv8_decode", q, k_cache, v_cache, k_scale, v_scale, block_table, tok_pos, tok_seq, True, 1, max_kv_len, num_kv_heads, scale, window, out, sink, keep_first, slopes, n_splits)
+    into (`n_splits` sets it where keys are streamed: 1 to 8 ranges, or 0, all keys of the step dealt out over one wave of CTAs).
+    `window`, `sink`, `keep_first`, `slopes`: see `attention_rows`.  A row whose position is negative or beyond its sequence's row of the
+    table is left as it is in `out`."""
+    return _attend("attention_kv8_decode", q, k_cache, v_cache, k_scale, v_scale, block_table, tok_pos, tok_seq, True, 1, max_kv_len,
+                   num_kv_heads, scale, window, out, sink, keep_first, slopes, n_splits)
 
 
 def attention_kv8_prefill(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, k_scale: torch.Tensor,
@@ -317,5 +325,5 @@ def attention_kv8_prefill(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch
     """Causal attention of every sequence's new tokens (rows seq_start[b] .. seq_start[b + 1] of q [T, H, hd], at most `max_new`) over
     its keys 0 .. seq_kv_len[b] - 1 (at most `max_kv_len`) in the 8-bit cache; returns [T, H * hd].  Rows of no sequence are left as they
     are in `out`.  The rest as in `attention_kv8_decode`."""
-    return _attend("attention_kv8_prefill", q, k_cache, v_cache, k_scale, v_scale, block_table, seq_start, seq_kv_len, False, max_new, max_kv_len, num_kv_heads, scale, window, out, sink,
-                   keep_first, slopes, n_splits)
+    return _attend("attention_kv8_prefill", q, k_cache, v_cache, k_scale, v_scale, block_table, seq_start, seq_kv_len, False, max_new, max_kv_len,
+                   num_kv_heads, scale, window, out, sink, keep_first, slopes, n_splits)

@@ -333,3 +333,71 @@ def test_queries_of_any_magnitude(level):
     scale = hd ** -0.5 / level
     got = ops.attention_kv8_decode(q.to(DEV), s.dk, s.dv, s.dks, s.dvs, i32([99, 80, 64]), i32([0, 1, 2]), s.dt, 100, G, scale)
     check_attention(got, s, q, [(0, 0, 99), (1, 1, 80), (2, 2, 64)], G, scale, "bfloat16")
+
+
+@pytest.mark.parametrize("dtype", ["bfloat16", "float32"])
+@pytest.mark.parametrize("H,G,hd", [(8, 2, 64), (16, 1, 128), (4, 2, 80), (2, 2, 24)])
+def test_rows_whose_scores_are_all_nan_or_all_minus_infinity(H, G, hd, dtype):
+    """A range of keys that has nothing but a NaN must not pass for an empty one, and a softmax of minus infinities is NaN, or nothing
+    beside a sink."""
+    from picolm_b200 import ops
+    n = 65                                                            # one key on the second page, and that one is NaN
+    s = Setup([n, 300, 3], G, hd, seed=2).fill([n, 300, 3], G, hd)
+    s.k[int(s.table[0, 1]), :, 0, 0] = 0x7f
+    s.k[:, :, :, 1] = 0x38                                            # (1.0)
+    s.device()
+    q = torch.randn((4, H, hd), generator=s.g).to(DTYPES[dtype])
+    q[1, 0, 2] = math.nan                                             # a query that is NaN
+    q[2, 1, 1] = -math.inf                                            # scores that are -inf
+    sink = torch.randn(H, generator=s.g)
+    pos, seq = [64, 299, 299, 2], [0, 1, 1, 2]
+    for more in (None, sink):
+        on = None if more is None else more.to(DEV)
+        for splits in (None, 0, 1, 3, 8):
+            got = ops.attention_kv8_decode(q.to(DEV), s.dk, s.dv, s.dks, s.dvs, i32(pos), i32(seq), s.dt, 300, G, hd ** -0.5, n_splits=splits, sink=on)
+            check_attention(got, s, q, [(t, seq[t], pos[t]) for t in range(4)], G, hd ** -0.5, dtype, sink=more)
+            assert bool(got[0].isnan().all()) and bool((got.view(4, H, hd)[2, 1] == 0).all()) == (more is not None)
+    # prompts: the same keys and queries among others, few rows and many
+    for new in (4, 60):
+        s = Setup([130 + new], G, hd, seed=new).fill([130 + new], G, hd)
+        s.k[:, :, :, 1] = 0x38
+        s.k[int(s.table[0, (129 + new) // PAGE]), :, (129 + new) % PAGE, 0] = 0xff
+        s.device()
+        q = torch.randn((new, H, hd), generator=s.g).to(DTYPES[dtype])
+        q[1, 0, 2], q[2, 1, 1] = math.nan, -math.inf
+        for more in (None, sink):
+            for window in (None, 1):
+                got = ops.attention_kv8_prefill(q.to(DEV), s.dk, s.dv, s.dks, s.dvs, i32([0, new]), i32([130 + new]), s.dt, new, 130 + new, G, hd ** -0.5,
+                                                window=window, sink=None if more is None else more.to(DEV))
+                check_attention(got, s, q, [(i, 0, 130 + i) for i in range(new)], G, hd ** -0.5, dtype, sink=more, window=window)
+
+
+def test_bounds_far_beyond_what_a_table_holds():
+    """keep_first, window, max_new and max_kv_len that pass 32 bits mean all that there is."""
+    from picolm_b200 import ops
+    H, G, hd, n, far = 4, 2, 64, 70, 1 << 40
+    s = Setup([100 + n], G, hd, seed=1).fill([100 + n], G, hd).device()
+    q = torch.randn((n, H, hd), generator=s.g)
+    for dtype in ("bfloat16", "float32"):
+        x = q.to(DTYPES[dtype])
+        for new in (2, n):
+            start, kv = i32([0, new]), i32([100 + new])
+            for more in (dict(window=far), dict(window=-far), dict(window=9, keep_first=far), dict(keep_first=2 ** 31 - 1, window=2 ** 31 - 1)):
+                got = ops.attention_kv8_prefill(x[:new].to(DEV), s.dk, s.dv, s.dks, s.dvs, start, kv, s.dt, far, far, G, 0.125, **more)
+                check_attention(got, s, x, [(i, 0, 100 + i) for i in range(0, new, 11)], G, 0.125, dtype)
+        got = ops.attention_kv8_decode(x[:3].to(DEV), s.dk, s.dv, s.dks, s.dvs, i32([0, 99, 169]), i32([0, 0, 0]), s.dt, far, G, 0.125, window=far)
+        check_attention(got, s, x, [(0, 0, 0), (1, 0, 99), (2, 0, 169)], G, 0.125, dtype)
+
+
+def test_more_new_tokens_than_the_sequence_is_long():
+    """Nothing is written for it, wherever its first position would be."""
+    from picolm_b200 import ops
+    H, G, hd = 2, 1, 64
+    s = Setup([100, 100], G, hd, seed=6).fill([100, 100], G, hd).device()
+    before = [x.clone() for x in (s.dk.view(torch.uint8), s.dv.view(torch.uint8), s.dks, s.dvs)]
+    for kv in (0, 1, 20, 70):
+        qkv = torch.randn((80, (H + 2 * G) * hd), generator=s.g).bfloat16().to(DEV)
+        q = torch.full((80, H, hd), 7.0, dtype=torch.bfloat16, device=DEV)
+        ops.rope_store_kv8(qkv, q, s.dk, s.dv, s.dks, s.dvs, None, None, i32([0, 0, 80]), i32([100, kv]), s.dt, 80, H, G, hd, 0, "half")
+        assert bool((q == 7.0).all())
+    assert all(torch.equal(a, b) for a, b in zip(before, (s.dk.view(torch.uint8), s.dv.view(torch.uint8), s.dks, s.dvs)))
