@@ -196,18 +196,23 @@ def kv8_cluster_splits(ctas: int, at_once: int, max_kv_len: int) -> int:
 
 
 def kv8_streams(walks: int, rows: int, max_kv_len: int, head_dim: int) -> bool:
-    """Whether prompts of at most `rows` (token, head) rows a sequence and kv head, `walks` of those, have their keys streamed (32 rows
-    at a time, the keys cut among CTAs) or take a CTA for 256 rows that walks all of them.  By what the two take a page: the tcgen05
-    kernel about 1 us whatever the rows, the streaming one 0.9 us of an SM for 32 rows of heads of 128 (0.4 of 64) and 10 more to begin
-    and join.  us, streamed / not, 32 heads over 8 of 128: 16 sequences of 9 tokens behind 3,000 75 / 49; one of 4, 16 and 40 behind
-    8,000 16 / 106, 53 / 106, 79 / 144."""
+    """Whether prompts of at most `rows` (token, head) rows a sequence and kv head, `walks` of those, have their keys streamed (16 or 32
+    rows at a time, the keys cut among CTAs) or take a CTA for 128 or 256 rows that walks all of them.  By what the two take, in us: the
+    tcgen05 kernel 7 to begin and end and 0.6 a page for 128 rows (heads of 64: 0.54), 1.0 for 256; the streaming one 10 and 0.5 of an
+    SM (0.25) a page for up to 16 rows, for 32 0.9 and 30 (0.4 and 12).  us, streamed / not, 32 heads over 8 of 128: 16 sequences
+    of 4 tokens behind 3,000 31 / 36, of 9 77 / 37; one of 16 behind 8,000 53 / 81, behind 1,000 32 / 17; of 64: 8 of 10 behind
+    4,000 31 / 40, 16 of 9 behind 3,000 40 / 32."""
     if head_dim not in (64, 128):
         return rows <= KV8_FEW_ROWS
     if rows > KV8_FEW_ROWS_MOST:
         return False
     pages = -(-max_kv_len // PAGE_TOKENS)
-    streamed = 10 + walks * -(-rows // 32) * pages * (0.9 if head_dim == 128 else 0.4) / SM_COUNT
-    return streamed < -(-walks // SM_COUNT) * pages
+    start, page = ((10, 0.5) if rows <= 16 else (30, 0.9)) if head_dim == 128 else ((10, 0.25) if rows <= 16 else (12, 0.4))
+    streamed = start + walks * -(-rows // 32) * pages * page / SM_COUNT
+    ctas, a_page = walks * -(-rows // 128), 0.6 if head_dim == 128 else 0.54
+    if rows > 128 and ctas > SM_COUNT:
+        ctas, a_page = walks, 1.0
+    return streamed < max(1.0, ctas / SM_COUNT) * (7 + pages * a_page)
 
 
 _variants = {}
@@ -276,7 +281,7 @@ def _attend(what, q, k_cache, v_cache, k_scale, v_scale, block_table, first, sec
             _bounds("kv8", (), k_cache, block_table)
         code = _fn("kv8", "plm_kv8_attention_rows")(q.data_ptr(), dtype, *cache, _p(ws), *step, table, pages, T, B, max_new, H, G, hd, *masks, splits, *rest)
         _launched(code, lambda: f"{what} T={T} H={H} G={G} hd={hd} rows splits={splits}", 1 if ws is None else 2, *need)
-    elif decode or kv8_streams(B * G, rows, seen, hd):
+    elif decode or (kv8_streams(B * G, rows, seen, hd) if n_splits is None else rows <= KV8_FEW_ROWS_MOST):
         lib, flags = _variant(hd, "attention_kv8")
         if CHECKED:
             _bounds(lib, flags, k_cache, block_table)
@@ -310,7 +315,7 @@ def attention_kv8_decode(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.
                          slopes: Optional[torch.Tensor] = None, n_splits: Optional[int] = None) -> torch.Tensor:
     """Attention of single query tokens (one per row of q [T, H, hd], at position tok_pos[t] of sequence tok_seq[t]) over the 8-bit
     cache; returns [T, H * hd].  `max_kv_len`: an upper bound of tok_pos + 1, for the choice of how many ranges the keys are cut
-    into (`n_splits` sets it where keys are streamed: 1 to 8 ranges, or 0, all keys of the step dealt out over one wave of CTAs).
+    into (`n_splits` sets it: 1 to 8 ranges, or 0, all keys of the step dealt out over one wave of CTAs).
     `window`, `sink`, `keep_first`, `slopes`: see `attention_rows`.  A row whose position is negative or beyond its sequence's row of the
     table is left as it is in `out`."""
     return _attend("attention_kv8_decode", q, k_cache, v_cache, k_scale, v_scale, block_table, tok_pos, tok_seq, True, 1, max_kv_len,
@@ -324,6 +329,7 @@ def attention_kv8_prefill(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch
                           slopes: Optional[torch.Tensor] = None, n_splits: Optional[int] = None) -> torch.Tensor:
     """Causal attention of every sequence's new tokens (rows seq_start[b] .. seq_start[b + 1] of q [T, H, hd], at most `max_new`) over
     its keys 0 .. seq_kv_len[b] - 1 (at most `max_kv_len`) in the 8-bit cache; returns [T, H * hd].  Rows of no sequence are left as they
-    are in `out`.  The rest as in `attention_kv8_decode`."""
+    are in `out`.  `n_splits`: for at most KV8_FEW_ROWS_MOST rows a sequence and kv head (new tokens times the heads of a group), that
+    keys are streamed, and in how many ranges.  The rest as in `attention_kv8_decode`."""
     return _attend("attention_kv8_prefill", q, k_cache, v_cache, k_scale, v_scale, block_table, seq_start, seq_kv_len, False, max_new, max_kv_len,
                    num_kv_heads, scale, window, out, sink, keep_first, slopes, n_splits)
