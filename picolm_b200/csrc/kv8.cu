@@ -94,7 +94,10 @@ template <int N> struct Angles {
 // prompts (an item is up to 64 rows, a CTA; what a thread loads stays in its registers until the scale is known), 1 for a few
 // tokens a sequence (four items a CTA).  EVEN: a row's units divide the item's threads, so that a thread has one place in a row
 // and every so many rows (no division on the way).
-// One read of the projection, one write of what it becomes: bound by memory for prompts, by the launch for single tokens.
+// One read of the projection, one write of what it becomes: bound by memory for prompts, by the launch for single tokens.  Measured (us,
+// what it reads within the L2): a prompt of 2,048, 32 heads over 8 of 64 6.7 (3.5 TB/s), 7 sequences of 1,011 in float32, 15 heads over 5
+// of 80 with 40 rotated 19.1 (3.3 TB/s), 64 single tokens 3.3, one 2.7.  A page's warps read, meet for its scale and write, with one wave
+// of items an SM and half.  16 bytes a load and four query heads an item: a prompt of 8,192 39 -> 30.
 constexpr int Q_HEADS = 4;
 template <int N> struct Held { enum : int { UNITS = N == 8 ? 2 : 4 }; };      // units that a thread keeps between the two passes; more are read again
 template <typename T, int N, int W, bool EVEN>
@@ -270,7 +273,8 @@ int append(const Append& a, int n_seqs, int max_new, cudaStream_t stream) {
 // A CTA of four warps takes WARPS * RPW (token, query head) rows of one sequence and kv head, RPW a warp, and a range of the
 // keys that any of them sees, 32 at a time: keys and values as floats in shared memory (number * scale is exact there), a lane
 // a key for the scores, a lane VEC components for the sums; running maximum and sum a row.  The ranges' partial results
-// (sum, maximum, denominator) meet in kv8_merge_kernel.
+// (sum, maximum, denominator) meet in kv8_merge_kernel.  Bound by shared memory: four products a lane cost nine 16-byte reads for eight
+// rows.  Measured: two prompts of 301 tokens, 32 heads over 8 of 64 59 us (9 TFLOP/s).
 constexpr int WARPS = 4;
 
 template <bool V> struct Const { static constexpr bool value = V; };
