@@ -271,25 +271,27 @@ int append(const Append& a, int n_seqs, int max_new, cudaStream_t stream) {
 
 // ------------------------------------------------------------------------------------------------ attention, fp32
 // A CTA of four warps takes WARPS * RPW (token, query head) rows of one sequence and kv head, RPW a warp, and a range of the
-// keys that any of them sees, 32 at a time: keys and values as floats in shared memory (number * scale is exact there), a lane
-// a key for the scores, a lane VEC components for the sums; running maximum and sum a row.  The ranges' partial results
-// (sum, maximum, denominator) meet in kv8_merge_kernel.  Bound by shared memory: four products a lane cost nine 16-byte reads for eight
-// rows.  Measured: two prompts of 301 tokens, 32 heads over 8 of 64 59 us (9 TFLOP/s).
+// keys that any of them sees, a group of 32 or (eight rows a warp) 64 at a time: keys and values as floats in shared memory (number * scale is
+// exact there), a lane one or two keys for the scores, a lane VEC components for the sums; running maximum a row, its sum in each lane's part.  The ranges' partial results
+// (sum, maximum, denominator) meet in kv8_merge_kernel.  Bound by shared memory: for eight rows and two keys 64 products a
+// lane take ten 16-byte reads (with one key nine for 32: 59 us where 52 are now).  Measured: two prompts of 301 tokens, 32 heads over 8 of 64
+// 52 us (10.6 TFLOP/s).
 constexpr int WARPS = 4;
 
 template <bool V> struct Const { static constexpr bool value = V; };
+__host__ __device__ constexpr int keys_a_lane(int rows_a_warp) { return rows_a_warp > 1 ? 2 : 1; }
 
 template <typename T, int RPW, int VEC>
 __global__ void __launch_bounds__(WARPS * 32)
 kv8_rows_kernel(const T* q, const uint8_t* kc, const uint8_t* vc, const float* ksc, const float* vsc, T* __restrict__ out,
                 float* __restrict__ ws, const Kv8Step step, int H, int G, int hd, float scale_log2, int window, int n_splits,
                 const float* sink, int keep, const float* slopes) {
-    constexpr int ROWS = WARPS * RPW, WIDE = 32 * VEC;
+    constexpr int ROWS = WARPS * RPW, WIDE = 32 * VEC, KPL = keys_a_lane(RPW), KG = 32 * KPL;
     extern __shared__ __align__(16) float sm[];
-    float* ks = sm;                                  // [32][hd + 4]
-    float* vs = ks + 32 * (hd + 4);                  // [32][WIDE], zero from hd on
-    float* qs = vs + 32 * WIDE;                      // [ROWS][hd]
-    float* ps = qs + ROWS * hd;                      // [ROWS][32]
+    float* ks = sm;                                  // [KG][hd + 4]
+    float* vs = ks + KG * (hd + 4);                  // [KG][WIDE], zero from hd on
+    float* qs = vs + KG * WIDE;                      // [ROWS][hd]
+    float* ps = qs + ROWS * hd;                      // [ROWS][KG]
     pdl_wait();
     pdl_launch_dependents();
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, R = H / G;
@@ -300,9 +302,9 @@ kv8_rows_kernel(const T* q, const uint8_t* kc, const uint8_t* vc, const float* k
     const long n_pairs = (long)sq.n_new * R, pair0 = ((n_pairs + ROWS - 1) / ROWS - 1 - (long)(lin / gridDim.y)) * ROWS;
     if (pair0 < 0) return;
     const int pos_first = sq.pos0 + (int)(pair0 / R), pos_last = sq.pos0 + (int)(min(pair0 + ROWS, n_pairs) - 1) / R;
-    // the walk: kept first positions that lie before the window's first group of 32, then the window's
-    const int lo0 = plm_first_key(pos_first, window), g_lo = lo0 / 32;
-    const int n_kept = min((keep + 31) / 32, g_lo), n_groups = n_kept + pos_last / 32 - g_lo + 1;
+    // the walk: kept first positions that lie before the window's first group, then the window's
+    const int lo0 = plm_first_key(pos_first, window), g_lo = lo0 / KG;
+    const int n_kept = min((keep + KG - 1) / KG, g_lo), n_groups = n_kept + pos_last / KG - g_lo + 1;
     const int per = (n_groups + n_splits - 1) / n_splits, w0 = split * per, w1 = min(n_groups, w0 + per);
 
     const int quads = hd / 4;
@@ -312,7 +314,7 @@ kv8_rows_kernel(const T* q, const uint8_t* kc, const uint8_t* vc, const float* k
         if (pair < n_pairs) load_group<T, 4>(q + ((sq.t0 + pair / R) * H + g * R + pair % R) * hd + i % quads * 4, x);
         *reinterpret_cast<float4*>(qs + i * 4) = make_float4(x[0], x[1], x[2], x[3]);
     }
-    for (int i = threadIdx.x; i < 32 * (WIDE - hd); i += WARPS * 32) vs[i / (WIDE - hd) * WIDE + hd + i % (WIDE - hd)] = 0.f;
+    for (int i = threadIdx.x; i < KG * (WIDE - hd); i += WARPS * 32) vs[i / (WIDE - hd) * WIDE + hd + i % (WIDE - hd)] = 0.f;
 
     float acc[RPW][VEC], m[RPW], l[RPW], slope[RPW];
     int pos[RPW], lo[RPW];
@@ -328,13 +330,13 @@ kv8_rows_kernel(const T* q, const uint8_t* kc, const uint8_t* vc, const float* k
         for (int i = 0; i < VEC; ++i) acc[r][i] = 0.f;
     }
     for (int w = w0; w < w1; ++w) {
-        const int key0 = (w < n_kept ? w : g_lo + w - n_kept) * 32;
+        const int key0 = (w < n_kept ? w : g_lo + w - n_kept) * KG;
         const int page = PLM_PAGE_NO(sq.pages[key0 / PLM_PAGE]);
         const size_t base = (((size_t)page * G + g) * PLM_PAGE + key0 % PLM_PAGE) * hd;
         const float sk = ksc[(size_t)page * G + g], sv = vsc[(size_t)page * G + g];
         __syncthreads();                                             // what was there has been read (and q is there)
         bool nan = false;
-        for (int i = threadIdx.x; i < 32 * quads; i += WARPS * 32) {
+        for (int i = threadIdx.x; i < KG * quads; i += WARPS * 32) {
             const int j = i / quads, c = i % quads * 4;
             float4 kv = make_float4(0.f, 0.f, 0.f, 0.f), vv = kv;
             if (key0 + j <= pos_last) {                              // (places behind hold whatever an earlier owner left)
@@ -350,40 +352,56 @@ kv8_rows_kernel(const T* q, const uint8_t* kc, const uint8_t* vc, const float* k
             *reinterpret_cast<float4*>(vs + j * WIDE + c) = vv;
         }
         nan = __syncthreads_or(nan);
-        float dot[RPW];
+        float dot[KPL][RPW];
 #pragma unroll
-        for (int r = 0; r < RPW; ++r) dot[r] = 0.f;
+        for (int n = 0; n < KPL; ++n)
+#pragma unroll
+            for (int r = 0; r < RPW; ++r) dot[n][r] = 0.f;
         const float* kr = ks + lane * (hd + 4);
 #pragma unroll 4
         for (int c = 0; c < hd; c += 4) {
-            const float4 k4 = *reinterpret_cast<const float4*>(kr + c);
+            float4 k4[KPL];
+#pragma unroll
+            for (int n = 0; n < KPL; ++n) k4[n] = *reinterpret_cast<const float4*>(kr + n * 32 * (hd + 4) + c);
 #pragma unroll
             for (int r = 0; r < RPW; ++r) {
                 const float4 q4 = *reinterpret_cast<const float4*>(qs + (r * WARPS + warp) * hd + c);
-                dot[r] = fmaf(q4.x, k4.x, fmaf(q4.y, k4.y, fmaf(q4.z, k4.z, fmaf(q4.w, k4.w, dot[r]))));
+#pragma unroll
+                for (int n = 0; n < KPL; ++n)
+                    dot[n][r] = fmaf(q4.x, k4[n].x, fmaf(q4.y, k4[n].y, fmaf(q4.z, k4[n].z, fmaf(q4.w, k4[n].w, dot[n][r]))));
             }
         }
-        const int key = key0 + lane;
 #pragma unroll
         for (int r = 0; r < RPW; ++r) {
-            const bool ok = key <= pos[r] && (key >= lo[r] || key < keep);
-            const float s = ok ? fmaf(slope[r], (float)(key - pos[r]), dot[r] * scale_log2) : -INFINITY;
-            const float m_new = fmaxf(m[r], warp_max(s)), m_use = m_new == -INFINITY ? 0.f : m_new;
-            const float down = exp2f(m[r] - m_use), p = exp2f(s - m_use);
-            l[r] = fmaf(l[r], down, warp_sum(p));
+            float most = -INFINITY;
+#pragma unroll
+            for (int n = 0; n < KPL; ++n) {
+                const int key = key0 + n * 32 + lane;
+                const bool ok = key <= pos[r] && (key >= lo[r] || key < keep);
+                dot[n][r] = ok ? fmaf(slope[r], (float)(key - pos[r]), dot[n][r] * scale_log2) : -INFINITY;
+                most = fmaxf(most, dot[n][r]);
+            }
+            const float m_new = fmaxf(m[r], warp_max(most)), m_use = m_new == -INFINITY ? 0.f : m_new;
+            const float down = exp2f(m[r] - m_use);
+            l[r] *= down;
             m[r] = m_new;
 #pragma unroll
             for (int i = 0; i < VEC; ++i) acc[r][i] *= down;
-            ps[(r * WARPS + warp) * 32 + lane] = p;
+#pragma unroll
+            for (int n = 0; n < KPL; ++n) {
+                const float p = exp2f(dot[n][r] - m_use);
+                l[r] += p;
+                ps[(r * WARPS + warp) * KG + n * 32 + lane] = p;
+            }
         }
         __syncwarp();
         // NAN: a masked key's value may be NaN; it is not looked at (0 * NaN)
         auto add = [&](auto skips) {
 #pragma unroll 2
-            for (int j0 = 0; j0 < 32; j0 += 4) {
+            for (int j0 = 0; j0 < KG; j0 += 4) {
                 float4 p4[RPW];
 #pragma unroll
-                for (int r = 0; r < RPW; ++r) p4[r] = *reinterpret_cast<const float4*>(ps + (r * WARPS + warp) * 32 + j0);
+                for (int r = 0; r < RPW; ++r) p4[r] = *reinterpret_cast<const float4*>(ps + (r * WARPS + warp) * KG + j0);
 #pragma unroll
                 for (int k = 0; k < 4; ++k) {
                     float v[VEC];
@@ -407,7 +425,8 @@ kv8_rows_kernel(const T* q, const uint8_t* kc, const uint8_t* vc, const float* k
 #pragma unroll
     for (int r = 0; r < RPW; ++r) {
         const long pair = pair0 + r * WARPS + warp;
-        if (pair >= n_pairs) continue;
+        if (pair >= n_pairs) continue;                               // (the whole warp)
+        l[r] = warp_sum(l[r]);
         const size_t row = (sq.t0 + pair / R) * H + g * R + pair % R;
         const float inv = n_splits > 1 ? 1.f : kv8_inverse(m[r], l[r], sink ? sink + g * R + pair % R : nullptr);
 #pragma unroll
@@ -452,7 +471,10 @@ kv8_merge_kernel(const float* ws, T* __restrict__ out, const Kv8Step step, int n
     }
 }
 
-size_t rows_smem(int rows, int wide, int hd) { return (size_t)(32 * (hd + 4) + 32 * wide + rows * hd + rows * 32) * sizeof(float); }
+size_t rows_smem(int rows, int wide, int hd) {
+    const int group = 32 * keys_a_lane(rows / WARPS);
+    return (size_t)(group * (hd + 4) + group * wide + rows * hd + rows * group) * sizeof(float);
+}
 
 template <typename T, int RPW, int VEC>
 int rows_launch(dim3 grid, const void* q, const void* kc, const void* vc, const float* ks, const float* vs, void* out, float* ws,
