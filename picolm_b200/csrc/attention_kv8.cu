@@ -16,13 +16,14 @@
 //                      (token, head) rows on its 8 columns, so that a group of four or eight heads does not leave half of the
 //                      MMA empty: S^T = K Q^T, and out^T = V^T P^T, whose A operand takes pairs of keys a component; a
 //                      byte permutation and a conversion make it of four rows of V.  The 8 columns of S^T become the
-//                      B operand by movmatrix.  Four warps' partial results meet in shared memory; CTAs' in their cluster's
-//                      where a step is small, else through a workspace and a second kernel, all keys of a step being dealt
-//                      out evenly over one wave of CTAs.
-//                      Measured, 32 heads over 8 (us, of the copy rate): 8 tokens behind 32,768 keys of 128 69.6, 0.81; 64 behind
-//                      4,096 of 64 39.7, 0.65; one behind 2,001 of 64 5.8 (a launch that reads almost nothing takes 4.5).
-//                      The cache in 16 bits takes 126, 60 and 6.  What a step waits for beside its bytes is the
-//                      second kernel, some 6 us with its start.  16 keys cost a warp 228 instructions.
+//                      B operand by movmatrix.  Four warps' partial results meet in shared memory; CTAs' in their cluster's,
+//                      or (few walks of long contexts) through a workspace and a second kernel, all keys of a step being
+//                      dealt out evenly over one wave of CTAs.
+//                      Measured, 32 heads over 8 (us, of the copy rate): 8 tokens behind 32,768 keys of 128 70, 0.81; 64 behind
+//                      4,096 of 64 37, 0.70; one behind 2,001 of 64 5.8 (a launch that reads almost nothing takes 4.5).
+//                      The cache in 16 bits takes 126, 60 and 6.  What a step waits for beside its bytes: in clusters the
+//                      CTAs' starts and meetings, some 1 us of an SM each, dealt out the second kernel, some 6 us with its
+//                      start.  16 keys cost a warp 228 instructions.
 //   kv8_tile_kernel    prompts of head sizes that the tcgen05 kernel does not take: 64 rows a CTA, pages of 64 keys brought to
 //                      shared memory as halves.
 #include "kv8.cuh"

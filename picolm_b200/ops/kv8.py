@@ -184,15 +184,26 @@ def kv8_few_plan(head_dim: int, rows: int):
     return plan
 
 
-def kv8_cluster_splits(ctas: int, at_once: int, max_kv_len: int) -> int:
+def kv8_cluster_splits(ctas: int, at_once: int, max_kv_len: int, head_dim: int, tile: int = 8) -> int:
     """Into how many ranges, the CTAs of a cluster, the streaming kernel cuts the keys of each sequence, for `ctas` CTAs without
-    cutting and `at_once` that run at once; 0: the keys of the step are dealt out over one wave of CTAs.  Dealing out costs a second
-    kernel and a longer start, some 6 us, and pays where the ranges would be longer than 16 pages or the CTAs more than run at once
-    (us, clusters / dealt out, 32 heads over 8: one sequence of 8,000 keys of 64 8.1 / 14.0, one of 32,000 of 128 26.6 / 24.8; 16 of 2,000
-    of 64 9.9 / 16.3, 64 of 1,000 of 128 30.1 / 27.5)."""
+    cutting, of `tile` rows, and `at_once` that run at once; 0: the keys of the step are dealt out over one wave of CTAs, which costs a
+    second kernel and a longer start, some 6 us.  As many ranges as run at once, where that leaves up to 64 pages to each; else, a CTA
+    costing some 1 us of an SM and the last ones' ranges the step's end, the square root of pages over CTAs (with the factor that was
+    best at 256 to 1,024 CTAs).  Dealt out where few walks leave most SMs without work for longer than the 6 us, and where CTAs of
+    more than 8 rows, which cost 2 to 4 us, do not run at once (40 sequences of 4 tokens behind 2,000 keys of 128 41 / 53).
+    us, dealt out / in 1, 2, 4, 8 ranges, 32 heads over 8, single tokens, unequal lengths up to the number: 64 sequences of 4,096 keys
+    of 64 40 / 40, 37, 44, -; of 16,384 121 / 136, 117, 107, -; 256 of 2,048 79 / 66, 78, 116, -; 8 of 16,384 26 / 61, 33, 24, 23;
+    64 of 4,096 of 128 68 / 70, 61, 68, -; 32 of 8,192 67 / 83, 72, 63, 71; one of 32,000 25 / -, -, -, 27."""
     pages = -(-max_kv_len // PAGE_TOKENS)
-    splits = min(KV8_CLUSTER_SPLITS, at_once // ctas, max(1, pages // 2))
-    return splits if splits >= 1 and pages <= 16 * splits else 0
+    most, runs = max(1, min(KV8_CLUSTER_SPLITS, pages // 2)), at_once // ctas
+    splits = min(most, runs)
+    if tile > 8:
+        if runs < 1 or (splits < 2 and pages > 16):
+            return 0
+    elif splits < 2 or pages > 64 * splits:
+        splits = min(most, max(1, round((31 * pages / ctas) ** 0.5)))
+    page = head_dim / 330                                 # us a CTA that has an SM to itself
+    return 0 if ctas * splits < at_once and pages / splits * page > 6.5 + pages * ctas / at_once * page else splits
 
 
 def kv8_streams(walks: int, rows: int, max_kv_len: int, head_dim: int) -> bool:
@@ -287,7 +298,7 @@ def _attend(what, q, k_cache, v_cache, k_scale, v_scale, block_table, first, sec
             _bounds(lib, flags, k_cache, block_table)
         tile, at_once, floats = kv8_few_plan(hd, rows)
         walks = B * G * -(-rows // tile)
-        splits = kv8_cluster_splits(walks, at_once, seen) if n_splits is None else n_splits
+        splits = kv8_cluster_splits(walks, at_once, seen, hd, tile) if n_splits is None else n_splits
         ws = None if splits else torch.empty((at_once * floats + 2 * walks,), dtype=torch.float32, device=q.device)
         code = _fn(lib, "plm_kv8_attention_few", flags)(q.data_ptr(), *cache, _p(ws), *step, table, pages, T, B, max_new, H, G, *masks, splits, at_once,
                                                         *rest)
