@@ -616,9 +616,15 @@ kv8_stream_kernel(const bf16* q, const Cache cache, bf16* __restrict__ out, floa
                 acc = fmaf(wgt, part[((size_t)w * COLS + col) * ROW + d], acc);
                 ll = fmaf(wgt, part[((size_t)w * COLS + col) * ROW + HD + 1], ll);
             }
+            if (n_splits == 1) {                                                   // nobody to meet
+                const int pair = pair0 + col, h = g * R + pair % R;
+                out[((size_t)(sq.t0 + pair / R) * H + h) * HD + d] = __float2bfloat16_rn(acc * kv8_inverse(mm, ll, sink ? sink + h : nullptr));
+                continue;
+            }
             mine[col * ROW + d] = acc;
             if (d == 0) { mine[col * ROW + HD] = mm; mine[col * ROW + HD + 1] = ll; }
         }
+        if (n_splits == 1) return;
         cluster_sync_all();
         for (int i = rank * NT + threadIdx.x; i < n_cols * HD; i += n_splits * NT) {
             const int col = i / HD, d = i - col * HD, pair = pair0 + col;

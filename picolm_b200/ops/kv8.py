@@ -192,8 +192,8 @@ def kv8_cluster_splits(ctas: int, at_once: int, max_kv_len: int, head_dim: int, 
     best at 256 to 1,024 CTAs).  Dealt out where few walks leave most SMs without work for longer than the 6 us, and where CTAs of
     more than 8 rows, which cost 2 to 4 us, do not run at once (40 sequences of 4 tokens behind 2,000 keys of 128 41 / 53).
     us, dealt out / in 1, 2, 4, 8 ranges, 32 heads over 8, single tokens, unequal lengths up to the number: 64 sequences of 4,096 keys
-    of 64 40 / 40, 37, 44, -; of 16,384 121 / 136, 117, 107, -; 256 of 2,048 79 / 66, 78, 116, -; 8 of 16,384 26 / 61, 33, 24, 23;
-    64 of 4,096 of 128 68 / 70, 61, 68, -; 32 of 8,192 67 / 83, 72, 63, 71; one of 32,000 25 / -, -, -, 27."""
+    of 64 40 / 39, 38, 44, 62; of 16,384 120 / 136, 117, 107, 115; 256 of 2,048 78 / 60, 78, 116, -; 8 of 16,384 26 / 61, 33, 24, 23;
+    64 of 4,096 of 128 68 / 64, 61, 68, 101; 32 of 8,192 67 / 81, 71, 63, 72; one of 32,000 25 / -, -, -, 27."""
     pages = -(-max_kv_len // PAGE_TOKENS)
     most, runs = max(1, min(KV8_CLUSTER_SPLITS, pages // 2)), at_once // ctas
     splits = min(most, runs)
