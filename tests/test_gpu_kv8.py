@@ -401,3 +401,36 @@ def test_more_new_tokens_than_the_sequence_is_long():
         ops.rope_store_kv8(qkv, q, s.dk, s.dv, s.dks, s.dvs, None, None, i32([0, 0, 80]), i32([100, kv]), s.dt, 80, H, G, hd, 0, "half")
         assert bool((q == 7.0).all())
     assert all(torch.equal(a, b) for a, b in zip(before, (s.dk.view(torch.uint8), s.dv.view(torch.uint8), s.dks, s.dvs)))
+
+
+@pytest.mark.parametrize("more", [{}, dict(window=50), dict(window=40, keep_first=70), dict(window=-32), dict(slopes=True, keep_first=3, window=90), dict(sink=True)],
+                         ids=["causal", "window", "kept", "chunks", "slopes", "sink"])
+@pytest.mark.parametrize("hd", [64, 128])
+def test_prompts_of_more_tiles_than_run_at_once(hd, more):
+    """Enough sequences that a tile of 256 rows is one CTA's (fewer take 128 rows a CTA), of unequal lengths, one without new tokens; a NaN
+    in one value and one key."""
+    from picolm_b200 import ops
+    H, G = 4, 2
+    seqs = [(70 + j % 5, 13 * j % 130) for j in range(38)] + [(0, 9), (129, 70)]
+    lens = [n + b for n, b in seqs]
+    s = Setup(lens, G, hd, seed=hd).fill(lens, G, hd)
+    s.v[int(s.table[3, 1]), 1, 10, 7], s.k[int(s.table[5, 1]), 0, 20, 2] = 0x7f, 0xff
+    s.vs *= 2.0 ** torch.randint(-12, 13, s.vs.shape, generator=s.g)
+    s.vs.clamp_(2.0 ** -60, 2.0 ** 40)
+    s.device()
+    offs = [0]
+    for n, _ in seqs:
+        offs.append(offs[-1] + n)
+    q = torch.randn((offs[-1] + 3, H, hd), generator=s.g).bfloat16()
+    args = dict(more)
+    if args.pop("sink", None):
+        args["sink"] = torch.randn(H, generator=s.g) * 2
+    if args.pop("slopes", None):
+        args["slopes"] = torch.rand(H, generator=s.g) * 0.1
+    on = {k: v.to(DEV) if isinstance(v, torch.Tensor) else v for k, v in args.items()}
+    out = torch.full((offs[-1] + 3, H * hd), 5.0, dtype=q.dtype, device=DEV)
+    ops.attention_kv8_prefill(q.to(DEV), s.dk, s.dv, s.dks, s.dvs, i32(offs), i32(lens), s.dt, 129, max(lens), G, hd ** -0.5, out=out, **on)
+    assert bool((out[offs[-1]:] == 5.0).all()), "rows of no sequence"
+    check_attention(out, s, q, [(offs[b] + i, b, before + i) for b, (n, before) in enumerate(seqs) for i in sorted({0, n // 3, 64, n - 1} & set(range(n)))],
+                    G, hd ** -0.5, "bfloat16", **args)
+    ops.check_status(DEV)
