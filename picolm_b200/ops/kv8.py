@@ -12,6 +12,7 @@ Errors.  A number held is within 2^-4 of the value, relative to it, or within 2^
 and fp32 sums (bfloat16 queries)."""
 from __future__ import annotations
 
+import functools
 from typing import Optional
 
 import torch
@@ -52,10 +53,11 @@ def _cache_check(what, k_cache, v_cache, k_scale, v_scale, G, hd, dev):
     if not kv8_supported(hd):
         raise KernelError(f"{what}: head_dim {hd} is not supported (a multiple of 8 up to {KV8_MAX_HEAD_DIM})")
     shape = k_cache.shape
-    if k_cache.dtype is not KV8_DTYPE or v_cache.dtype is not KV8_DTYPE or len(shape) != 4 or shape[1:] != (G, PAGE_TOKENS, hd) or v_cache.shape != shape:
+    held = (shape[0] if shape else 0, G)
+    if k_cache.dtype is not KV8_DTYPE or v_cache.dtype is not KV8_DTYPE or shape != (held[0], G, PAGE_TOKENS, hd) or v_cache.shape != shape:
         raise KernelError(f"{what}: k_cache and v_cache must be [pages, {G}, {PAGE_TOKENS}, {hd}] of {KV8_DTYPE}, got {k_cache.dtype} {tuple(shape)} and "
                           f"{v_cache.dtype} {tuple(v_cache.shape)}")
-    if k_scale.dtype is not torch.float32 or v_scale.dtype is not torch.float32 or k_scale.shape != shape[:2] or v_scale.shape != shape[:2]:
+    if k_scale.dtype is not torch.float32 or v_scale.dtype is not torch.float32 or k_scale.shape != held or v_scale.shape != held:
         raise KernelError(f"{what}: k_scale and v_scale must be float32 [{shape[0]}, {G}], got {k_scale.dtype} {tuple(k_scale.shape)} and "
                           f"{v_scale.dtype} {tuple(v_scale.shape)}")
 
@@ -89,6 +91,7 @@ def _bounds(library, flags, k_cache, table, n_table: int = 0) -> None:
 
 
 def _launched(code: int, say, kernels: int = 1, nbytes: int = 0, flops: int = 0) -> None:
+    """`_check` with a name that is put together only where it is looked at."""
     _check(code, say() if code or TRACED else "", kernels, nbytes, flops)
 
 
@@ -116,7 +119,8 @@ def _append(what, dev, T, q_at, k_at, v_at, dtype, item, lds, q_out, k_cache, v_
         n_table = shape[0]
     if T == 0:
         return
-    max_new = min(max_new, T)
+    if max_new > T:
+        max_new = T
     if CHECKED:
         _bounds("kv8", (), k_cache, block_table, n_table)
     code = _fn("kv8", "plm_kv8_append")(
@@ -184,8 +188,9 @@ def kv8_few_plan(head_dim: int, rows: int):
     return plan
 
 
-def kv8_cluster_splits(ctas: int, at_once: int, max_kv_len: int, head_dim: int, tile: int = 8) -> int:
-    """Into how many ranges, the CTAs of a cluster, the streaming kernel cuts the keys of each sequence, for `ctas` CTAs without
+@functools.lru_cache(maxsize=4096)
+def kv8_cluster_splits(ctas: int, at_once: int, pages: int, head_dim: int, tile: int = 8) -> int:
+    """Into how many ranges, the CTAs of a cluster, the streaming kernel cuts the `pages` of each sequence, for `ctas` CTAs without
     cutting, of `tile` rows, and `at_once` that run at once; 0: the keys of the step are dealt out over one wave of CTAs, which costs a
     second kernel and a longer start, some 6 us.  As many ranges as run at once, where that leaves up to 64 pages to each; else, a CTA
     costing some 1 us of an SM and the last ones' ranges the step's end, the square root of pages over CTAs (with the factor that was
@@ -194,7 +199,6 @@ def kv8_cluster_splits(ctas: int, at_once: int, max_kv_len: int, head_dim: int, 
     us, dealt out / in 1, 2, 4, 8 ranges, 32 heads over 8, single tokens, unequal lengths up to the number: 64 sequences of 4,096 keys
     of 64 40 / 39, 38, 44, 62; of 16,384 120 / 136, 117, 107, 115; 256 of 2,048 78 / 60, 78, 116, -; 8 of 16,384 26 / 61, 33, 24, 23;
     64 of 4,096 of 128 68 / 64, 61, 68, 101; 32 of 8,192 67 / 81, 71, 63, 72; one of 32,000 25 / -, -, -, 27."""
-    pages = -(-max_kv_len // PAGE_TOKENS)
     most, runs = max(1, min(KV8_CLUSTER_SPLITS, pages // 2)), at_once // ctas
     splits = min(most, runs)
     if tile > 8:
@@ -275,7 +279,9 @@ def _attend(what, q, k_cache, v_cache, k_scale, v_scale, block_table, first, sec
     # (no sequence brings more than all rows, none is longer than its row of the table)
     table, pages = block_table.data_ptr(), block_table.shape[1]
     held = pages * PAGE_TOKENS
-    max_new, max_kv_len, keep_first = min(int(max_new), T), max(1, min(int(max_kv_len), held)), min(int(keep_first), held)
+    max_new = T if max_new > T else int(max_new)
+    max_kv_len = held if max_kv_len > held else int(max_kv_len) if max_kv_len > 0 else 1
+    keep_first = min(int(keep_first), held) if keep_first else 0
     window = max(-held, min(int(window), held)) if window else 0
     step = (first.data_ptr(), second.data_ptr(), None, None) if decode else (None, None, first.data_ptr(), second.data_ptr())
     cache = (k_cache.data_ptr(), v_cache.data_ptr(), k_scale.data_ptr(), v_scale.data_ptr(), out.data_ptr())
@@ -298,7 +304,7 @@ def _attend(what, q, k_cache, v_cache, k_scale, v_scale, block_table, first, sec
             _bounds(lib, flags, k_cache, block_table)
         tile, at_once, floats = kv8_few_plan(hd, rows)
         walks = B * G * -(-rows // tile)
-        splits = kv8_cluster_splits(walks, at_once, seen, hd, tile) if n_splits is None else n_splits
+        splits = kv8_cluster_splits(walks, at_once, -(-seen // PAGE_TOKENS), hd, tile) if n_splits is None else n_splits
         ws = None if splits else torch.empty((at_once * floats + 2 * walks,), dtype=torch.float32, device=q.device)
         code = _fn(lib, "plm_kv8_attention_few", flags)(q.data_ptr(), *cache, _p(ws), *step, table, pages, T, B, max_new, H, G, *masks, splits, at_once,
                                                         *rest)

@@ -130,5 +130,5 @@ def test_the_number_of_ranges_is_one_that_the_kernel_takes(head_dim, at_once, ti
     from picolm_b200.ops.kv8 import KV8_CLUSTER_SPLITS, kv8_cluster_splits
     for ctas in (1, 3, 8, 64, 500, 2048, 65535 * 128):
         for keys in (1, 64, 65, 129, 1000, 4096, 33000, 2 ** 21, 2 ** 31 - 1):
-            n = kv8_cluster_splits(ctas, at_once, keys, head_dim, tile)
+            n = kv8_cluster_splits(ctas, at_once, -(-keys // 64), head_dim, tile)
             assert 0 <= n <= KV8_CLUSTER_SPLITS and n <= max(1, -(-keys // 64) // 2), (ctas, keys, n)
