@@ -1107,7 +1107,7 @@ extern "C" int plm_kv8_attention_few(const void* q, const void* kc, const void* 
     if (n_rows <= 0 || n_seqs <= 0 || max_new <= 0) return PLM_OK;
     if (H <= 0 || G <= 0 || H % G || n_seqs > 65535 || (ws ? n_ctas < 1 || n_ctas > MAX_CTAS : n_splits < 1 || n_splits > MAX_CLUSTER) || keep < 0) return PLM_ERR_SHAPE;
     if (bad_step(tok_pos, tok_seq, seq_start, seq_kv_len)) return PLM_ERR_UNSUPPORTED;
-    if (((uintptr_t)q | (uintptr_t)kc | (uintptr_t)vc) & 15) return PLM_ERR_ALIGN;
+    if (((uintptr_t)q | (uintptr_t)kc | (uintptr_t)vc) & 15 || (uintptr_t)out & 3) return PLM_ERR_ALIGN;      // (out: pairs of bf16)
     const Kv8Step step = {tok_pos, tok_seq, seq_start, seq_kv_len, block_table, max_pages};
     const Cache cache = {(const uint8_t*)kc, (const uint8_t*)vc, ks, vs};
     const int groups = groups_of((long)max_new * (H / G));
@@ -1126,7 +1126,7 @@ extern "C" int plm_kv8_attention_tiles(const void* q, const void* kc, const void
                                        const float* slopes, cudaStream_t s) {
     if (n_seqs <= 0 || max_new <= 0) return PLM_OK;
     if (H <= 0 || G <= 0 || H % G || n_seqs > 65535 || G > 65535 || keep < 0) return PLM_ERR_SHAPE;
-    if (((uintptr_t)q | (uintptr_t)kc | (uintptr_t)vc) & 15) return PLM_ERR_ALIGN;
+    if (((uintptr_t)q | (uintptr_t)kc | (uintptr_t)vc) & 15 || (uintptr_t)out & 3) return PLM_ERR_ALIGN;
     static std::atomic<unsigned long long> devices{0};
     cudaError_t e = plm_allow_smem(kv8_tile_kernel, TILE_SMEM, devices);
     if (e != cudaSuccess) return (int)e;

@@ -549,7 +549,7 @@ extern "C" int plm_kv8_attention_rows(const void* q, int dtype, const void* kc, 
     if (n_rows <= 0 || n_seqs <= 0 || max_new <= 0) return PLM_OK;
     if (H <= 0 || G <= 0 || H % G || hd <= 0 || hd % 8 || hd > 256 || n_splits < 1 || (n_splits > 1 && !ws) || keep < 0) return PLM_ERR_SHAPE;
     if (!tok_pos != !tok_seq || !tok_pos == !seq_start || !seq_start != !seq_kv_len) return PLM_ERR_UNSUPPORTED;
-    if ((uintptr_t)q & 15) return PLM_ERR_ALIGN;
+    if ((uintptr_t)q & 15 || ((uintptr_t)kc | (uintptr_t)vc) & 3) return PLM_ERR_ALIGN;      // (the caches: four bytes at a time)
     const Kv8Step step = {tok_pos, tok_seq, seq_start, seq_kv_len, block_table, max_pages};
     if (dtype == PLM_F32)
         return rows_any<float>(q, kc, vc, ks, vs, out, ws, step, n_seqs, max_new, H, G, hd, scale, window, n_splits, sink, keep, slopes, stream);

@@ -334,7 +334,8 @@ def attention_kv8_decode(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.
     cache; returns [T, H * hd].  `max_kv_len`: an upper bound of tok_pos + 1, for the choice of how many ranges the keys are cut
     into (`n_splits` sets it: 1 to 8 ranges, or 0, all keys of the step dealt out over one wave of CTAs).
     `window`, `sink`, `keep_first`, `slopes`: see `attention_rows`.  A row whose position is negative or beyond its sequence's row of the
-    table is left as it is in `out`."""
+    table is left as it is in `out`.  Tensors that begin off the boundary of the kernel's loads and stores (16 bytes; `out` of single tokens 4) are
+    refused."""
     return _attend("attention_kv8_decode", q, k_cache, v_cache, k_scale, v_scale, block_table, tok_pos, tok_seq, True, 1, max_kv_len,
                    num_kv_heads, scale, window, out, sink, keep_first, slopes, n_splits)
 
