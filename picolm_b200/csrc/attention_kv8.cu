@@ -6,7 +6,7 @@
 // over lo <= t <= p (or t < keep).  Every e4m3 number is a half; a query row becomes halves after a division by a power of two
 // that puts its largest number into [2^13, 2^14) (then halves hold every bit of what was within 2^27 of it); the scales, being
 // powers of two, stay outside the products: ks joins the factor on the scores, and the sum over values is kept in the unit
-// 2^eo of some page's vs: a page in another unit either has its weights multiplied by the ratio or, where that is beyond 2^6,
+// 2^eo of some page's vs: a page in another unit either has its weights multiplied by the ratio or, where that is beyond 2^KV8_SPAN,
 // changes the unit (a factor on the sums, exact).
 //
 // Two kernels:
@@ -41,8 +41,7 @@ constexpr int KS = HD / 16;                      // steps of the contraction ove
 constexpr int MT = HD / 16;                      // tiles of 16 components
 constexpr int VW = (HD / 8 + 3) / 4;             // words of a value's row in a lane
 constexpr int WARPS = 4, NT = 128;
-constexpr float RAISE = 8.f;                     // a row's maximum may outgrow its reference by 2^RAISE before sums are scaled
-constexpr int UNIT_SPAN = 6;                     // weights take a page's unit up to 2^6 from the sums'
+constexpr float LIFT = KV8_LIFT, RAISE = KV8_RAISE;
 
 __device__ __forceinline__ uint32_t smem_u32(const void* p) { return (uint32_t)__cvta_generic_to_shared(p); }
 __device__ __forceinline__ float ex2(float x) {
@@ -447,11 +446,11 @@ kv8_stream_kernel(const bf16* q, const Cache cache, bf16* __restrict__ out, floa
                     x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 4));
                     x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 8));
                     x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 16));
-                    mx[j][e] = x * c[j][e];                          // (c is positive)
+                    mx[j][e] = x * c[j][e] - LIFT;                   // (c is positive)
                     raise |= mx[j][e] > (m[j][e] == -INFINITY ? -INFINITY : m[j][e] + RAISE);
                 }
             int d = ev - eo;
-            if (__any_sync(0xffffffffu, raise || d > UNIT_SPAN || d < -UNIT_SPAN)) {
+            if (__any_sync(0xffffffffu, raise || d > KV8_SPAN || d < -KV8_SPAN)) {
 #pragma unroll
                 for (int j = 0; j < NG; ++j) {
                     float down[2];
@@ -981,7 +980,7 @@ kv8_tile_kernel(const bf16* q, const Cache cache, bf16* __restrict__ out, const 
             for (int hi = 0; hi < 2; ++hi) {
                 mx[hi] = fmaxf(mx[hi], __shfl_xor_sync(0xffffffffu, mx[hi], 1));
                 mx[hi] = fmaxf(mx[hi], __shfl_xor_sync(0xffffffffu, mx[hi], 2));
-                const float m_new = fmaxf(m[hi], mx[hi]);
+                const float m_new = fmaxf(m[hi], mx[hi] - LIFT);
                 use[hi] = m_new == -INFINITY ? 0.f : m_new;
                 l[hi] *= ex2(m[hi] - use[hi]);                                     // (-inf gives 0)
                 down[hi] = ex2(m[hi] - use[hi] + (float)(eo - ev));

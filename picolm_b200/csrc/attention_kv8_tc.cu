@@ -10,7 +10,7 @@
 //   softmax        a thread a row: its 64 scores out of tensor memory, running maximum and sum in fp32, probabilities as halves
 //                  over the first half of the scores' place
 //   O += P V       tcgen05.mma, P from tensor memory, V in shared memory (MN-major); O stays in tensor memory and is scaled only when
-//                  a row's maximum outgrows its reference by 2^8 or a page's values have a scale beyond 2^6 from O's unit
+//                  a row's maximum outgrows its reference or a page's values have a scale beyond 2^KV8_SPAN from O's unit
 // Warps 0..7 are the softmax threads of the two tiles (quarter = warp % 4), 8 and 9 make halves of keys' bytes, 10 and 11 of values',
 // 12 and 14 issue the tiles' MMAs (12 owns the tensor memory), 13 asks for pages: a page's keys and values of a kv head are
 // contiguous, so that each is one bulk copy of 4 or 8 KB into a ring of raw pages.  While one tile's threads work on page i, the
@@ -264,8 +264,6 @@ kv8_tc_kernel(const bf16* q, const Cache cache, bf16* __restrict__ out, const Kv
         const float slope2 = EXTRA && slopes ? slopes[head] * LOG2E : 0.f;
         const uint32_t lanes = (uint32_t)(quarter * 32) << 16;
         const uint32_t tm_o = tmem + lanes + TM_O + t * HD;
-        constexpr float RAISE = 8.f;
-        constexpr int UNIT_SPAN = 6;
         float m_ref = -INFINITY, l = 0.f;
         int eo = 0;
         bool ok = true;
@@ -331,10 +329,10 @@ kv8_tc_kernel(const bf16* q, const Cache cache, bf16* __restrict__ out, const Kv
                 mx3 = max3(mx3, __uint_as_float(s0[j + 3]), __uint_as_float(s1[j + 3]));
             }
             mx = fmaxf(fmaxf(mx, mx1), fmaxf(mx2, mx3));
-            const float m_cand = fmaxf(m_ref, mx * c2);                            // (c2 is positive)
+            const float m_cand = fmaxf(m_ref, mx * c2 - (float)KV8_LIFT);          // (c2 is positive)
             int d = ev - eo;
-            const bool raise = m_cand > (m_ref == -INFINITY ? -INFINITY : m_ref + RAISE);
-            if (__any_sync(0xffffffffu, raise || d > UNIT_SPAN || d < -UNIT_SPAN)) {                // tcgen05.ld/st are warp-wide
+            const bool raise = m_cand > (m_ref == -INFINITY ? -INFINITY : m_ref + (float)KV8_RAISE);
+            if (__any_sync(0xffffffffu, raise || d > KV8_SPAN || d < -KV8_SPAN)) {                // tcgen05.ld/st are warp-wide
                 const float by = raise ? m_ref - m_cand : 0.f;                     // -inf where nothing was seen before
                 if (i > 0) {
                     // O may only be touched once every P V issued so far has landed in it

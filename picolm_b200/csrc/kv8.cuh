@@ -5,12 +5,23 @@
 // finite magnitude that the page holds (448 is e4m3's largest number).  What a place holds is number * scale; a value that is not finite
 // is held as NaN, one beyond 448 * 2^KV8_E_MAX as that.  With scales that are powers of two a page whose scale has to grow
 // keeps what it holds: its numbers' exponents shift, and only those that become subnormal (below 2^-6) are rounded again.
-// The bounds of e keep 2^(e - e') of any two pages and sums in the unit of either inside float32.
+// The bounds of e keep 2^(e - e') of any two pages inside float32, and sums over numbers (below 2^9) times weights (below 2^12,
+// see KV8_LIFT) in the unit of a page 2^80 below theirs for up to 2^27 keys; in a unit 2^100 below for 2^7 at the least.
 #pragma once
 #include "common.cuh"
 #include <cuda_fp16.h>
 
 constexpr int KV8_E_MIN = -60, KV8_E_MAX = 40;
+
+// Weights of bf16 attention are halves: exp2(score - reference) * 2^d.  The reference of a row lies 2^KV8_LIFT below its largest score so
+// far, and follows once that is 2^KV8_RAISE further up; d, of a page whose values are in another unit than the sums, is at most
+// KV8_SPAN, else the sums change their unit.  So a row's largest weight is at least 2^KV8_LIFT, no half passes 2^15, and a weight
+// has a half's 11 bits down to 2^-20 of the largest and is off by at most 2^-31 of that below.  With the largest at 1 (LIFT 0,
+// RAISE 8, SPAN 6) weights below 2^-25 of the largest were lost: where a first token draws the weight and holds next to
+// nothing, all that 3,000 others give.  Single tokens take the same time; prompts (us, so / as now): 2,048 of 64 41.8 / 42.4, 1,000
+// behind 15,000 of 128 274.4 / 275.6, 600 behind 3,000 69.7 / 70.5; with 7, 4, 4 42.9, 275.7, 71.1: sums are scaled more often.
+constexpr int KV8_LIFT = 6, KV8_RAISE = 6, KV8_SPAN = 3;
+static_assert(KV8_LIFT + KV8_RAISE + KV8_SPAN <= 15, "the largest half is below 2^16");
 
 // Two e4m3 numbers, the low byte's first, as halves (exact; NaN stays NaN).
 __device__ __forceinline__ uint32_t kv8_halves(uint32_t two) {

@@ -9,7 +9,7 @@ becomes subnormal is rounded again.  Page 0 is nobody's and is never written.
 
 Errors.  A number held is within 2^-4 of the value, relative to it, or within 2^-10 of its page's scale for values below
 2^-6 of that.  Attention works in fp32 over exactly what is held (float32 queries), or with queries and weights as halves
-and fp32 sums (bfloat16 queries)."""
+and fp32 sums (bfloat16 queries): weights to 2^-11 down to 2^-20 of a row's largest, below that to 2^-31 of the largest."""
 from __future__ import annotations
 
 import functools
