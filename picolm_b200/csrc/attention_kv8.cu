@@ -642,8 +642,7 @@ kv8_stream_kernel(const bf16* q, const Cache cache, bf16* __restrict__ out, floa
             float acc = 0.f, ll = 0.f;
 #pragma unroll
             for (int s = 0; s < MAX_CLUSTER; ++s) {
-                if (ms[s] == -INFINITY) continue;
-                const float wgt = exp2f(ms[s] - mm);
+                const float wgt = ms[s] == -INFINITY ? 0.f : exp2f(ms[s] - mm);    // (its sum is zero, or NaN where a value is)
                 acc = fmaf(wgt, as[s], acc);
                 ll = fmaf(wgt, ls[s], ll);
             }
@@ -724,19 +723,17 @@ kv8_join_kernel(const float* ws, const int2* pieces, bf16* __restrict__ out, con
             const bool have = i0 + i < who.y;
             const float* p = place(have ? i0 + i : i0);
             ms[i] = p[HD]; ls[i] = p[HD + 1]; as[i] = p[d];
-            if (!have) ms[i] = -INFINITY;
+            if (!have) { ms[i] = -INFINITY; as[i] = 0.f; }
         }
 #pragma unroll
         for (int i = 0; i < AT_ONCE; ++i) top = fmaxf(top, ms[i]);
-        if (top == -INFINITY) continue;
-        const float f = exp2f(m - top);
+        const float f = m == -INFINITY ? 0.f : exp2f(m - top);
         l *= f;
         acc *= f;
         m = top;
 #pragma unroll
         for (int i = 0; i < AT_ONCE; ++i) {
-            if (ms[i] == -INFINITY) continue;
-            const float w = exp2f(ms[i] - top);
+            const float w = ms[i] == -INFINITY ? 0.f : exp2f(ms[i] - top);         // (its sum is zero, or NaN where a value is)
             l = fmaf(w, ls[i], l);
             acc = fmaf(w, as[i], acc);
         }

@@ -395,7 +395,7 @@ kv8_rows_kernel(const T* q, const uint8_t* kc, const uint8_t* vc, const float* k
             }
         }
         __syncwarp();
-        // NAN: a masked key's value may be NaN; it is not looked at (0 * NaN)
+        // NaN among the values: it counts for the rows that see its place, whatever their weight, and for no others (0 * NaN)
         auto add = [&](auto skips) {
 #pragma unroll 2
             for (int j0 = 0; j0 < KG; j0 += 4) {
@@ -413,8 +413,10 @@ kv8_rows_kernel(const T* q, const uint8_t* kc, const uint8_t* vc, const float* k
 #pragma unroll
                     for (int r = 0; r < RPW; ++r) {
                         const float p = k == 0 ? p4[r].x : k == 1 ? p4[r].y : k == 2 ? p4[r].z : p4[r].w;
+                        const int key = key0 + j0 + k;
+                        const bool skip = decltype(skips)::value && !(key <= pos[r] && (key >= lo[r] || key < keep));
 #pragma unroll
-                        for (int i = 0; i < VEC; ++i) acc[r][i] = fmaf(p, decltype(skips)::value && p == 0.f ? 0.f : v[i], acc[r][i]);
+                        for (int i = 0; i < VEC; ++i) acc[r][i] = fmaf(p, skip ? 0.f : v[i], acc[r][i]);
                     }
                 }
             }
@@ -465,7 +467,7 @@ kv8_merge_kernel(const float* ws, T* __restrict__ out, const Kv8Step step, int n
         float acc = 0.f;
         for (int s = 0; s < n_splits; ++s) {
             const float ms = p[(size_t)s * (hd + 2) + hd];
-            if (ms != -INFINITY) acc = fmaf(exp2f(ms - m), p[(size_t)s * (hd + 2) + d], acc);
+            acc = fmaf(ms == -INFINITY ? 0.f : exp2f(ms - m), p[(size_t)s * (hd + 2) + d], acc);       // (its sum is zero, or NaN where a value is)
         }
         out[row * hd + d] = from_f32<T>(acc * inv);
     }

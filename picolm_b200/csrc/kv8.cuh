@@ -89,8 +89,8 @@ __device__ __forceinline__ Kv8Seq kv8_seq(const Kv8Step& s, int b) {
     return q;
 }
 
-// The maximum that a partial result goes by where several are put together: ones with -inf are skipped as empty, and a NaN among the scores,
-// which is in l and not in the maximum, must not be.
+// The maximum that a partial result goes by where several are put together: ones with -inf have no weight, and a NaN among the scores,
+// which is in l and not in the maximum, must have one.
 __device__ __forceinline__ float kv8_top(float m, float l) { return l == l ? m : fmaxf(m, 0.f); }
 
 // With a sink (one more term exp(sink) in the denominator) the factor that turns a row's sum_j exp2(s_j - m) v_j into its
