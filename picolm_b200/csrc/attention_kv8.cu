@@ -186,18 +186,26 @@ struct Walk {
 constexpr int MAX_CLUSTER = 8;
 constexpr int MAX_CTAS = 6 * PLM_SM_COUNT;       // (a float a warp fits the second kernel's shared memory)
 constexpr int ROW = HD + 2;                      // floats of a partial result's row: sums, maximum, denominator
+constexpr int SM_SMEM = 228 * 1024;              // shared memory of an SM
+// (CTAS, an SM: what registers allow, and shared memory by one unit less in the ring where it must, in both forms of the kernel: heads of
+// 112 with three CTAs of two units / two of three 57 / 64 us for 64 sequences of 4,096; two rows' groups of 32 of heads of 128 and of 16 of 240
+// share an SM since a CTA's sums lie over its first warp's: 8 sequences of 8,192 keys with 32 rows 39 -> 31, with 16 of 240 46 -> 38.)
 template <int NG> struct Few {
     enum : int {
         SB = HD * NG <= 256 && HD <= 128 ? 2 : 1,                    // blocks of 16 keys at a time
         KB = 16 * SB,
         TILE = KB * HD,                                              // bytes of KB keys
-        STAGES = TILE >= 4096 ? 2 : TILE >= 2048 ? 3 : 4,            // units a warp has in its ring
         CTAS = NG == 1 ? (HD <= 64 ? 4 : HD <= 128 ? 3 : 2) : NG == 2 && HD <= 64 ? 3 : 2,      // an SM
         Q_BYTES = NG > 1 ? WARPS * NG * KS * 32 * 8 : 0,             // the queries' fragments (of one group: in registers)
+        AFTER = (WARPS * ROW + 2) * 8 * NG * 4,                      // the warps' results; what a CTA shows to its cluster: in the first's place
+        SLACK = 1024 + 128,                                          // a CTA's beside: the system's, what the kernel declares itself
+        MOST = SM_SMEM / CTAS - SLACK - Q_BYTES,                     // of a CTA for its ring
+        WANTED = TILE >= 4096 ? 2 : TILE >= 2048 ? 3 : 4,
+        STAGES = WARPS * WANTED * 2 * TILE <= MOST ? WANTED : WANTED - 1,                       // units a warp has in its ring
         RING = WARPS * STAGES * 2 * TILE,
-        AFTER = (WARPS + 1) * 8 * NG * ROW * 4,                      // the warps' results, what a CTA shows to its cluster
         SMEM = Q_BYTES + (RING > AFTER ? (int)RING : (int)AFTER),
     };
+    static_assert(STAGES >= 2 && CTAS * (SMEM + SLACK) <= SM_SMEM, "as many CTAs an SM as the work is dealt out to");
 };
 
 // The rows of one sequence and kv head, COLS at a time, against its keys: how the work is dealt out.  A sequence's walk is one of
@@ -583,7 +591,8 @@ kv8_stream_kernel(const bf16* q, const Cache cache, bf16* __restrict__ out, floa
     const Deal<COLS, KB> deal = {step, n_seqs, G, R, window, keep, tiles};
     if constexpr (CLUSTER) {
         float* part = reinterpret_cast<float*>(sm_raw + Few<NG>::Q_BYTES);         // after the walk, in the rings' place: [WARPS][COLS][ROW]
-        float* mine = part + WARPS * COLS * ROW;                                   // [COLS][ROW]
+        float* mine = part;                                                        // [COLS][ROW], each number where the one thread that needs it
+        float* tops = part + WARPS * COLS * ROW;                                   // had the first warp's; [COLS][2] maximum and denominator
         const int g = blockIdx.y / tiles, tile = blockIdx.y - g * tiles, n_splits = gridDim.x, rank = blockIdx.x;
         const Kv8Seq sq = kv8_seq(step, blockIdx.z);
         int units, n_tiles;
@@ -621,7 +630,7 @@ kv8_stream_kernel(const bf16* q, const Cache cache, bf16* __restrict__ out, floa
                 continue;
             }
             mine[col * ROW + d] = acc;
-            if (d == 0) { mine[col * ROW + HD] = mm; mine[col * ROW + HD + 1] = ll; }
+            if (d == 0) { tops[col * 2] = mm; tops[col * 2 + 1] = ll; }
         }
         if (n_splits == 1) return;
         cluster_sync_all();
@@ -632,10 +641,10 @@ kv8_stream_kernel(const bf16* q, const Cache cache, bf16* __restrict__ out, floa
             for (int s = 0; s < MAX_CLUSTER; ++s) {
                 ms[s] = -INFINITY; ls[s] = 0.f; as[s] = 0.f;
                 if (s < n_splits) {
-                    const uint32_t at = cluster_map(mine + col * ROW, (uint32_t)s);
-                    ms[s] = cluster_ld_f32(at + HD * 4);
-                    ls[s] = cluster_ld_f32(at + (HD + 1) * 4);
-                    as[s] = cluster_ld_f32(at + d * 4);
+                    const uint32_t top = cluster_map(tops + col * 2, (uint32_t)s);
+                    ms[s] = cluster_ld_f32(top);
+                    ls[s] = cluster_ld_f32(top + 4);
+                    as[s] = cluster_ld_f32(cluster_map(mine + col * ROW + d, (uint32_t)s));
                 }
                 mm = fmaxf(mm, ms[s]);
             }
@@ -1086,7 +1095,10 @@ bool bad_step(const int* tok_pos, const int* tok_seq, const int* seq_start, cons
 // for every sequence, kv head and tile of that many rows.
 extern "C" int plm_kv8_few_ctas(int rows) {
     const int ng = groups_of(rows);
-    return PLM_SM_COUNT * (ng == 1 ? (int)Few<1>::CTAS : ng == 2 ? (int)Few<2>::CTAS : (int)Few<4>::CTAS);
+#if PLM_HD <= 128
+    if (ng == 4) return PLM_SM_COUNT * (int)Few<4>::CTAS;
+#endif
+    return PLM_SM_COUNT * (ng == 1 ? (int)Few<1>::CTAS : (int)Few<2>::CTAS);
 }
 extern "C" int plm_kv8_few_floats(int rows) { return WARPS * 2 * 8 * groups_of(rows) * ROW; }
 extern "C" int plm_kv8_few_tile(int rows) { return 8 * groups_of(rows); }
@@ -1109,8 +1121,10 @@ extern "C" int plm_kv8_attention_few(const void* q, const void* kc, const void* 
     const int groups = groups_of((long)max_new * (H / G));
     if (groups == 1) return stream<1>((const bf16*)q, cache, (bf16*)out, ws, step, n_seqs, max_new, H, G, scale, window, n_splits, n_ctas, sink, keep, slopes, s);
     if (groups == 2) return stream<2>((const bf16*)q, cache, (bf16*)out, ws, step, n_seqs, max_new, H, G, scale, window, n_splits, n_ctas, sink, keep, slopes, s);
-    if constexpr (HD <= 128)
+#if PLM_HD <= 128
+    if (groups == 4)
         return stream<4>((const bf16*)q, cache, (bf16*)out, ws, step, n_seqs, max_new, H, G, scale, window, n_splits, n_ctas, sink, keep, slopes, s);
+#endif
     return PLM_ERR_UNSUPPORTED;
 }
 

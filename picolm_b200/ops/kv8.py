@@ -195,15 +195,19 @@ def kv8_cluster_splits(ctas: int, at_once: int, pages: int, head_dim: int, tile:
     second kernel and a longer start, some 6 us.  As many ranges as run at once, where that leaves up to 64 pages to each; else, a CTA
     costing some 1 us of an SM and the last ones' ranges the step's end, the square root of pages over CTAs (with the factor that was
     best at 256 to 1,024 CTAs).  Dealt out where few walks leave most SMs without work for longer than the 6 us, and where CTAs of
-    more than 8 rows, which cost 2 to 4 us, do not run at once (40 sequences of 4 tokens behind 2,000 keys of 128 41 / 53).
+    more than 8 rows, which cost 2 to 4 us, do not run at once and have walks that are long enough (40 sequences of 4 tokens, 32 heads over 8,
+    behind 2,000 keys of 128 42 / 47, of 64 31 / 28; 64 of 8 behind 1,000 of 64 55 / 43).
     us, dealt out / in 1, 2, 4, 8 ranges, 32 heads over 8, single tokens, unequal lengths up to the number: 64 sequences of 4,096 keys
-    of 64 40 / 39, 38, 44, 62; of 16,384 120 / 136, 117, 107, 115; 256 of 2,048 78 / 60, 78, 116, -; 8 of 16,384 26 / 61, 33, 24, 23;
-    64 of 4,096 of 128 68 / 64, 61, 68, 101; 32 of 8,192 67 / 81, 71, 63, 72; one of 32,000 25 / -, -, -, 27."""
+    of 64 41 / 39, 38, 45, 63; of 16,384 121 / 135, 118, 109, 117; 256 of 2,048 79 / 61, 80, 120, 190; 8 of 16,384 27 / 62, 35, 25, 24;
+    64 of 4,096 of 128 68 / 64, 62, 69, 102; 32 of 8,192 68 / 76, 71, 64, 73; one of 32,000 23 / 166, 87, 47, 27.  Of 112: 64 of 4,096 61 / 58, 57, 66,
+    99; 8 of 32,768 64 / 163, 86, 71, 67.  Other heads (8 over 1, 16 over 2, 64 and 128 over 8, 32 over 32, 6 over 6), 1 to 200 sequences of
+    1,000 to 60,000: what is chosen takes at most 1.13 of the best."""
     most, runs = max(1, min(KV8_CLUSTER_SPLITS, pages // 2)), at_once // ctas
     splits = min(most, runs)
     if tile > 8:
-        if runs < 1 or (splits < 2 and pages > 16):
+        if splits < 2 and pages * head_dim > 2500:
             return 0
+        splits = max(1, splits)
     elif splits < 2 or pages > 64 * splits:
         splits = min(most, max(1, round((31 * pages / ctas) ** 0.5)))
     page = head_dim / 330                                 # us a CTA that has an SM to itself
@@ -214,15 +218,15 @@ def kv8_streams(walks: int, rows: int, max_kv_len: int, head_dim: int) -> bool:
     """Whether prompts of at most `rows` (token, head) rows a sequence and kv head, `walks` of those, have their keys streamed (16 or 32
     rows at a time, the keys cut among CTAs) or take a CTA for 128 or 256 rows that walks all of them.  By what the two take, in us: the
     tcgen05 kernel 7 to begin and end and 0.6 a page for 128 rows (heads of 64: 0.54), 1.0 for 256; the streaming one 10 and 0.5 of an
-    SM (0.25) a page for up to 16 rows, for 32 0.9 and 30 (0.4 and 12).  us, streamed / not, 32 heads over 8 of 128: 16 sequences
-    of 4 tokens behind 3,000 31 / 36, of 9 77 / 37; one of 16 behind 8,000 53 / 81, behind 1,000 32 / 17; of 64: 8 of 10 behind
-    4,000 31 / 40, 16 of 9 behind 3,000 40 / 32."""
+    SM (0.25) a page for up to 16 rows, for 32 20 and 0.72 (12 and 0.5).  us, streamed / not, 32 heads over 8 of 128: 16 sequences
+    of 4 tokens behind 3,000 31 / 36, of 8 51 / 37, 64 of 8 behind 1,000 67 / 55; one of 16 behind 8,000 34 / 81, of 8 behind 1,000 18 / 17; of 64: 4 of 8 behind
+    4,000 18 / 41, 16 of 8 behind 3,000 33 / 33, of 16 46 / 34; 16 heads over 2 of 128, 16 of 4 behind 3,000 23 / 35, 40 behind 2,000 40 / 27."""
     if head_dim not in (64, 128):
         return rows <= KV8_FEW_ROWS
     if rows > KV8_FEW_ROWS_MOST:
         return False
     pages = -(-max_kv_len // PAGE_TOKENS)
-    start, page = ((10, 0.5) if rows <= 16 else (30, 0.9)) if head_dim == 128 else ((10, 0.25) if rows <= 16 else (12, 0.4))
+    start, page = ((10, 0.5) if rows <= 16 else (20, 0.72)) if head_dim == 128 else ((10, 0.25) if rows <= 16 else (12, 0.5))
     streamed = start + walks * -(-rows // 32) * pages * page / SM_COUNT
     ctas, a_page = walks * -(-rows // 128), 0.6 if head_dim == 128 else 0.54
     if rows > 128 and ctas > SM_COUNT:
