@@ -4,7 +4,8 @@
 // [pages, G], a power of two 2^e with KV8_E_MIN <= e <= KV8_E_MAX: the smallest with 448 * 2^e at or above the largest
 // finite magnitude that the page holds (448 is e4m3's largest number).  What a place holds is number * scale; a value that is not finite
 // is held as NaN, one beyond 448 * 2^KV8_E_MAX as that.  With scales that are powers of two a page whose scale has to grow
-// keeps what it holds: its numbers' exponents shift, and only those that become subnormal (below 2^-6) are rounded again.
+// keeps what it holds: its numbers' exponents shift, and only those that become subnormal (below 2^-6) are rounded again: off by
+// 2^-10 of the scale as they come, by less than 2^-9 of it after any number of growths.
 // The bounds of e keep 2^(e - e') of any two pages inside float32, and sums over numbers (below 2^9) times weights (below 2^12,
 // see KV8_LIFT) in the unit of a page 2^80 below theirs for up to 2^27 keys; in a unit 2^100 below for 2^7 at the least.
 #pragma once

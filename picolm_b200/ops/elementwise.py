@@ -316,7 +316,8 @@ def qk_norm_rope_store(qkv: torch.Tensor, bias: Optional[torch.Tensor], q_norm: 
     its scores.  `conv` (float32 [taps, columns of qkv], tap-major, the token's own tap last; no bias with it): every
     column is first convolved over time with the sequence's projected rows before; `conv_state` (float32 [slots + 1,
     >= (taps - 1) * columns], contiguous rows) holds every sequence's last taps - 1 projected rows, oldest first, and
-    is brought up to date.  A cache in 8 bits (`kv.k_scale`) takes the keys and values by a kernel of its own behind this one."""
+    is brought up to date.  A cache in 8 bits (`kv.k_scale`) takes the keys and values by a kernel of its own behind this one, from
+    rows of q_out's type: in bfloat16 they are rounded to it first, as a cache in 16 bits holds them, and to 8 bits then."""
     if not qkv.is_cuda or qkv.dim() != 2 or qkv.stride(1) != 1:
         raise KernelError("qk_norm_rope_store: qkv must be a matrix with contiguous rows on the device")
     _dev(q_out, "q_out")

@@ -8,7 +8,9 @@ page whose scale has to grow because of a later token keeps what it holds: its n
 becomes subnormal is rounded again.  Page 0 is nobody's and is never written.
 
 Errors.  A number held is within 2^-4 of the value, relative to it, or within 2^-10 of its page's scale for values below
-2^-6 of that.  Attention works in fp32 over exactly what is held (float32 queries), or with queries and weights as halves
+2^-6 of that; of a page whose scale has grown since it came, within 2^-9 of the scale (every growth rounds what is subnormal
+once more, and the scale at least doubles: 2^-10 (1 + 1/2 + ..)).  Keys and values that `qk_norm_rope_store` hands over (heads that
+are normed, biased or convolved) are rows of the run's type: in a bfloat16 run rounded to that, 2^-9, before.  Attention works in fp32 over exactly what is held (float32 queries), or with queries and weights as halves
 and fp32 sums (bfloat16 queries): weights to 2^-11 down to 2^-20 of a row's largest, below that to 2^-31 of the largest."""
 from __future__ import annotations
 
