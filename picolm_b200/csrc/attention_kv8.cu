@@ -388,8 +388,8 @@ kv8_stream_kernel(const bf16* q, const Cache cache, bf16* __restrict__ out, floa
                 for (int j = 0; j < NG; ++j) s[b][j][0] = s[b][j][1] = s[b][j][2] = s[b][j][3] = 0.f;
             cp_wait<2 * STAGES - 1>();                               // this unit's keys are there
             __syncwarp();
-            const float ks_now = scales[warp][stage][0];
-            const int ev = kv8_exponent_of_scale(scales[warp][stage][1]);
+            const float ks_now = kv8_scale(scales[warp][stage][0]);
+            const int ev = kv8_exponent_of_scale(kv8_scale(scales[warp][stage][1]));
             uint32_t kw[SB][2][KS];
 #pragma unroll
             for (int b = 0; b < SB; ++b) {
@@ -882,8 +882,8 @@ kv8_tile_kernel(const bf16* q, const Cache cache, bf16* __restrict__ out, const 
     auto base_of = [&](int i) { return ((size_t)PLM_PAGE_NO(sq.pages[walk.page_at(i)]) * G + g); };
     auto ask = [&](int i) {
         const size_t at = base_of(i);
-        ks = cache.ks[at];
-        vs = cache.vs[at];
+        ks = kv8_scale(cache.ks[at]);
+        vs = kv8_scale(cache.vs[at]);
         if (AHEAD) {
 #pragma unroll
             for (int c = 0; c < CHUNKS; ++c) {

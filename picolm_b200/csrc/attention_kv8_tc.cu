@@ -272,8 +272,8 @@ kv8_tc_kernel(const bf16* q, const Cache cache, bf16* __restrict__ out, const Kv
         if (my_pages > 0) {
             const size_t at = (size_t)PLM_PAGE_NO(sq.pages[page_at(i_first)]) * G + g;
             page_next = sq.pages[page_at(i_first + i_step * min(1, my_pages - 1))];
-            ks_next = cache.ks[at];
-            vs_next = cache.vs[at];
+            ks_next = kv8_scale(cache.ks[at]);
+            vs_next = kv8_scale(cache.vs[at]);
             eo = kv8_exponent_of_scale(vs_next);
         }
         for (int i = 0; i < my_pages && ok; ++i) {
@@ -281,8 +281,8 @@ kv8_tc_kernel(const bf16* q, const Cache cache, bf16* __restrict__ out, const Kv
             const int ev = kv8_exponent_of_scale(vs_next);
             if (i + 1 < my_pages) {
                 const size_t at = (size_t)PLM_PAGE_NO(page_next) * G + g;
-                ks_next = cache.ks[at];
-                vs_next = cache.vs[at];
+                ks_next = kv8_scale(cache.ks[at]);
+                vs_next = kv8_scale(cache.vs[at]);
                 page_next = sq.pages[page_at(i_first + i_step * min(i + 2, my_pages - 1))];
             }
             const uint32_t s_tm = tmem + lanes + TM_S + t * 128 + (i & 1) * 64;

@@ -165,7 +165,7 @@ kv8_append_kernel(const Append a) {
     float* scale_at = (key ? a.ks : a.vs) + (size_t)page * a.G + g;
     const bool rotate = key && a.cos_t != nullptr;
     const int place = first % PLM_PAGE;                          // rows before it are there already
-    const int e_old = place ? kv8_exponent_of_scale(*scale_at) : KV8_E_MIN;
+    const int e_old = place ? kv8_exponent_of_scale(kv8_scale(*scale_at)) : KV8_E_MIN;
 
     auto read = [&](int j, float* x) {
         const int r = row_of(j);
@@ -333,7 +333,7 @@ kv8_rows_kernel(const T* q, const uint8_t* kc, const uint8_t* vc, const float* k
         const int key0 = (w < n_kept ? w : g_lo + w - n_kept) * KG;
         const int page = PLM_PAGE_NO(sq.pages[key0 / PLM_PAGE]);
         const size_t base = (((size_t)page * G + g) * PLM_PAGE + key0 % PLM_PAGE) * hd;
-        const float sk = ksc[(size_t)page * G + g], sv = vsc[(size_t)page * G + g];
+        const float sk = kv8_scale(ksc[(size_t)page * G + g]), sv = kv8_scale(vsc[(size_t)page * G + g]);
         __syncthreads();                                             // what was there has been read (and q is there)
         bool nan = false;
         for (int i = threadIdx.x; i < KG * quads; i += WARPS * 32) {

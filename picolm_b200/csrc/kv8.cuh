@@ -59,6 +59,18 @@ __device__ __forceinline__ int kv8_exponent(float a) {
     return min(max(e, KV8_E_MIN), KV8_E_MAX);
 }
 __device__ __forceinline__ float kv8_pow2(int e) { return __int_as_float((e + 127) << 23); }      // -126 <= e <= 127
+// A page's scale as a kernel reads it: the sums go by its exponent alone, so one that is no power of two, or out of bounds, would give
+// other results in bfloat16 than in float32.  The checked build records it.
+#ifdef PLM_CHECK
+__device__ __forceinline__ float kv8_scale(float s) {
+    const uint32_t bits = __float_as_uint(s);
+    if (!(bits & 0x807fffffu) && bits >= (uint32_t)(KV8_E_MIN + 127) << 23 && bits <= (uint32_t)(KV8_E_MAX + 127) << 23) return s;
+    if (plm_bounds.status) atomicCAS(plm_bounds.status, 0, 20);
+    return 1.f;
+}
+#else
+__device__ __forceinline__ float kv8_scale(float s) { return s; }
+#endif
 __device__ __forceinline__ int kv8_exponent_of_scale(float s) { return (int)(__float_as_uint(s) >> 23) - 127; }
 
 // A step's sequence as attention sees it.  With tok_pos every row of q is a token of its own (`b` is its number), at

@@ -373,7 +373,7 @@ def set_bounds(library: str, extra_flags=(), *, n_pages: int = 0, n_seqs: int = 
 
 
 # What the status word says: what the checked build met (csrc/common.cuh), or whose wait ran out.
-_OUT_OF_BOUNDS = {16: "page number", 17: "sequence index", 18: "position", 19: "row index"}
+_OUT_OF_BOUNDS = {16: "page number", 17: "sequence index", 18: "position", 19: "row index", 20: "scale of a page"}
 _WAITS = {1: "TMA producer", 2: "MMA issuer", 3: "epilogue", 4: "the CTAs' meeting", 5: "a decode step's pages", 40: "the walk over chunks", 44: "the chunks' TMA producer", 45: "the chunks' MMA issuer",
           46: "the chunks' split", 47: "the chunks' sums", 48: "a retention chunk's products",
           41: "the experts' streamed weights", 42: "the experts' streamed products", 43: "the experts' streamed rows",

@@ -5,7 +5,8 @@ what is held, for single tokens and for prompts.
 What a place holds is its number times its page's scale.  A scale is the smallest 2^e, -60 <= e <= 40, with 448 * 2^e at or above the
 largest magnitude that its page holds (values beyond 448 * 2^40 are held as that, values that are not finite as NaN).  A
 page whose scale has to grow because of a later token keeps what it holds: its numbers' exponents shift, and only what
-becomes subnormal is rounded again.  Page 0 is nobody's and is never written.
+becomes subnormal is rounded again.  Page 0 is nobody's and is never written.  A cache made elsewhere must
+hold such scales too, no others: the kernels go by their exponents (the checked build reports one that is not).
 
 Errors.  A number held is within 2^-4 of the value, relative to it, or within 2^-10 of its page's scale for values below
 2^-6 of that; of a page whose scale has grown since it came, within 2^-9 of the scale (every growth rounds what is subnormal
