@@ -57,7 +57,7 @@ class Engine:
             for block in model.blocks:
                 for prefix, part in block.parts():
                     specs = part.cache_specs() if hasattr(part, "cache_specs") else [part.cache_spec()] if hasattr(part, "cache_spec") else []
-                    if any(sp is not None and sp.kind == "kv" and sp.values for sp in specs) and not part.takes_kv8:
+                    if any(sp is not None and sp.kind == "kv" and sp.values for sp in specs) and not getattr(part, "takes_kv8", False):
                         raise ValueError(f"cache type {cache_type!r}: the {part.family} {part.kind!r} keeps keys and values that this "
                                          f"cache does not take (heads of a multiple of 8 up to 256, written by a part that says takes_kv8)")
         self.cache = SequenceCache(model.cache_specs(), max_tokens=max_tokens,
