@@ -19,13 +19,15 @@
 //                      B operand by movmatrix.  Four warps' partial results meet in shared memory; CTAs' in their cluster's,
 //                      or (few walks of long contexts) through a workspace and a second kernel, all keys of a step being
 //                      dealt out evenly over one wave of CTAs.
-//                      Measured, 32 heads over 8 (us, of the copy rate): 8 tokens behind 32,768 keys of 128 70, 0.81; 64 behind
-//                      4,096 of 64 37, 0.70; one behind 2,001 of 64 5.8 (a launch that reads almost nothing takes 4.5).
+//                      Measured, 32 heads over 8 (us, of the copy rate): 8 tokens behind 32,768 keys of 128 72, 0.79; 64 behind
+//                      4,096 of 64 37, 0.69; one behind 2,001 of 64 6.0 (a launch that reads almost nothing takes 4.5).
 //                      The cache in 16 bits takes 126, 60 and 6.  What a step waits for beside its bytes: in clusters the
 //                      CTAs' starts and meetings, some 1 us of an SM each, dealt out the second kernel, some 6 us with its
 //                      start.  16 keys cost a warp 228 instructions.
 //   kv8_tile_kernel    prompts of head sizes that the tcgen05 kernel does not take: 64 rows a CTA, pages of 64 keys brought to
-//                      shared memory as halves.
+//                      shared memory as halves.  Measured, 32 heads over 8 (us): a prompt of 1,000 of 80 66 (0.05 of the bf16 rate), of
+//                      96 83, of 112 88, of 256 159; 500 behind 7,500 374, 342, 364, 893.  The legacy MMAs, and a page that every
+//                      CTA widens for its 64 rows, are what takes it.
 #include "kv8.cuh"
 
 #ifndef PLM_HD

@@ -21,7 +21,7 @@
 // and V 256, the conversion reads and writes 384), the 16,384 exponentials 1,024 of the special-function units, the products 1,024 of the
 // tensor cores; a page takes some 2,100.  Heads of 64: 700, 1,024, 512 of some 1,600.  The rest is hand-overs: a wait on a barrier that is
 // ready costs a warp 150 cycles here, a page is five of them in a row.  Measured, 32 heads over 8 of 128 (us): 1,000 tokens behind 15,000 keys
-// 274 (930 TFLOP/s), 2,048 of 64 41 (420), 16 sequences of 9 tokens behind 3,000 37.  What made it so, at the first of those: keys and
+// 276 (920 TFLOP/s), 2,048 of 64 42 (415), 16 sequences of 9 tokens behind 3,000 37.  What made it so, at the first of those: keys and
 // values converted by two teams that wait for nothing of each other, every load of a page asked for before any is used, one arrival a
 // warp and not one a thread, waits that park (polling threads take the issue slots that the conversion needs): 292 -> 274.
 // 128 rows a CTA, every other page a tile: where a wave holds all CTAs of 128 rows, or none has more (us, 256 rows / 128: 500 tokens

@@ -95,8 +95,9 @@ template <int N> struct Angles {
 // tokens a sequence (four items a CTA).  EVEN: a row's units divide the item's threads, so that a thread has one place in a row
 // and every so many rows (no division on the way).
 // One read of the projection, one write of what it becomes: bound by memory for prompts, by the launch for single tokens.  Measured (us,
-// what it reads within the L2): a prompt of 2,048, 32 heads over 8 of 64 6.7 (3.5 TB/s), 7 sequences of 1,011 in float32, 15 heads over 5
-// of 80 with 40 rotated 19.1 (3.3 TB/s), 64 single tokens 3.3, one 2.7.  A page's warps read, meet for its scale and write, with one wave
+// what it reads within the L2): a prompt of 2,048, 32 heads over 8 of 64 6.3 to 7.4 (9.9 from memory: 2.4 TB/s), 7 sequences of 1,011 in
+// float32, 15 heads over 5 of 80 with 40 rotated 19.3 (3.2 TB/s), 64 single tokens 3.2, one 2.6; where every open page's scale grows, and
+// what it holds is rounded again, 6.3 and 3.5.  A page's warps read, meet for its scale and write, with one wave
 // of items an SM and half.  16 bytes a load and four query heads an item: a prompt of 8,192 39 -> 30.
 constexpr int Q_HEADS = 4;
 template <int N> struct Held { enum : int { UNITS = N == 8 ? 2 : 4 }; };      // units that a thread keeps between the two passes; more are read again
@@ -273,9 +274,10 @@ int append(const Append& a, int n_seqs, int max_new, cudaStream_t stream) {
 // A CTA of four warps takes WARPS * RPW (token, query head) rows of one sequence and kv head, RPW a warp, and a range of the
 // keys that any of them sees, a group of 32 or (eight rows a warp) 64 at a time: keys and values as floats in shared memory (number * scale is
 // exact there), a lane one or two keys for the scores, a lane VEC components for the sums; running maximum a row, its sum in each lane's part.  The ranges' partial results
-// (sum, maximum, denominator) meet in kv8_merge_kernel.  Bound by shared memory: for eight rows and two keys 64 products a
-// lane take ten 16-byte reads (with one key nine for 32: 59 us where 52 are now).  Measured: two prompts of 301 tokens, 32 heads over 8 of 64
-// 52 us (10.6 TFLOP/s).
+// (sum, maximum, denominator) meet in kv8_merge_kernel.  For eight rows and two keys 64 products a lane take ten 16-byte reads (with one
+// key nine for 32: 59 us where 52 are now).  Measured: two prompts of 301 tokens, 32 heads over 8 of 64 52 us (10.6 TFLOP/s); no pipe is full
+// (FFMA 30 %, shared memory 31 %, 1.9 instructions a cycle): 12 warps an SM, which meet twice a group, with nothing asked for ahead.  The same
+// takes single tokens' time: one behind 2,001 keys 19 us, eight behind 4,096 52, eight behind 8,192 of 128 225 (their bytes: 0.3, 3.5, 14).
 constexpr int WARPS = 4;
 
 template <bool V> struct Const { static constexpr bool value = V; };
