@@ -24,7 +24,7 @@
 //                      The cache in 16 bits takes 126, 60 and 6.  What a step waits for beside its bytes: in clusters the
 //                      CTAs' starts and meetings, some 1 us of an SM each, dealt out the second kernel, some 6 us with its
 //                      start.  16 keys cost a warp 228 instructions.
-//   kv8_tile_kernel    prompts of head sizes that the tcgen05 kernel does not take: 64 rows a CTA, pages of 64 keys brought to
+//   kv8_tile_kernel    longer prompts of head sizes that the tcgen05 kernel does not take: 64 rows a CTA, pages of 64 keys brought to
 //                      shared memory as halves.  Measured, 32 heads over 8 (us): a prompt of 1,000 of 80 66 (0.05 of the bf16 rate), of
 //                      96 83, of 112 88, of 256 159; 500 behind 7,500 374, 342, 364, 893.  The legacy MMAs, and a page that every
 //                      CTA widens for its 64 rows, are what takes it.

@@ -175,7 +175,7 @@ def attention_kv8_mma_supported(q: torch.Tensor) -> bool:
 
 
 KV8_CLUSTER_SPLITS = 8          # up to this many ranges of keys meet inside a thread-block cluster, without scratch
-KV8_FEW_ROWS, KV8_FEW_ROWS_MOST = 64, 256          # (token, head) rows a sequence and kv head up to which keys may be streamed
+KV8_FEW_ROWS, KV8_FEW_ROWS_MOST = 64, 256          # (token, head) rows a sequence and kv head up to which keys are streamed in any case, or may be
 
 _few = {}
 
@@ -223,12 +223,17 @@ def kv8_streams(walks: int, rows: int, max_kv_len: int, head_dim: int) -> bool:
     tcgen05 kernel 7 to begin and end and 0.6 a page for 128 rows (heads of 64: 0.54), 1.0 for 256; the streaming one 10 and 0.5 of an
     SM (0.25) a page for up to 16 rows, for 32 20 and 0.72 (12 and 0.5).  us, streamed / not, 32 heads over 8 of 128: 16 sequences
     of 4 tokens behind 3,000 31 / 36, of 8 51 / 37, 64 of 8 behind 1,000 67 / 55; one of 16 behind 8,000 34 / 81, of 8 behind 1,000 18 / 17; of 64: 4 of 8 behind
-    4,000 18 / 41, 16 of 8 behind 3,000 33 / 33, of 16 46 / 34; 16 heads over 2 of 128, 16 of 4 behind 3,000 23 / 35, 40 behind 2,000 40 / 27."""
-    if head_dim not in (64, 128):
-        return rows <= KV8_FEW_ROWS
+    4,000 18 / 41, 16 of 8 behind 3,000 33 / 33, of 16 46 / 34; 16 heads over 2 of 128, 16 of 4 behind 3,000 23 / 35, 40 behind 2,000 40 / 27.
+    Other head sizes, whose tiles are 64 rows and leave the keys whole: up to KV8_FEW_ROWS rows always, above while there are at most 16
+    tiles a page (then both keep the SMs busy, and the streaming kernel's CTAs cost more to begin and to end).  us, streamed / not, 32 heads over 8
+    of 96: one of 32 behind 1,000 18 / 47, behind 8,000 32 / 279, of 64 47 / 280; 16 of 32 behind 3,000 87 / 140, behind 500 45 / 35; 64 of 64 behind
+    1,000 270 / 225; of 256: one of 32 behind 8,000 56 / 901, 64 behind 1,000 332 / 334; 16 heads over 2 of 80: 16 of 32 behind 3,000 51 / 114, 64 behind
+    1,000 71 / 60."""
     if rows > KV8_FEW_ROWS_MOST:
         return False
     pages = -(-max_kv_len // PAGE_TOKENS)
+    if head_dim not in (64, 128):
+        return rows <= KV8_FEW_ROWS or walks * -(-rows // 64) <= 16 * pages
     start, page = ((10, 0.5) if rows <= 16 else (20, 0.72)) if head_dim == 128 else ((10, 0.25) if rows <= 16 else (12, 0.5))
     streamed = start + walks * -(-rows // 32) * pages * page / SM_COUNT
     ctas, a_page = walks * -(-rows // 128), 0.6 if head_dim == 128 else 0.54
