@@ -68,3 +68,25 @@ def test_prompts(H, G, hd, new, octaves, spread):
         got = ops.attention_kv8_prefill(q.to(DEV), s.dk, s.dv, s.dks, s.dvs, i32([0, new]), i32([n]), s.dt, new, n, G, scale, **more)
         check(got, s, q, [(t, n - new + t) for t in sorted({0, 1, new // 2, new - 1})], G, scale, spread)
     ops.check_status(DEV)
+
+
+@pytest.mark.parametrize("low", [-40, -60])
+@pytest.mark.parametrize("H,G,hd,new", [(4, 2, 64, 1), (8, 1, 128, 1), (4, 2, 64, 300), (4, 1, 128, 7), (4, 2, 128, 70), (8, 2, 96, 100)])
+def test_units_as_far_apart_as_the_format_has_them(H, G, hd, new, low):
+    """Pages of values around 2^low and 2^40 in turn, with equal scores and with unequal ones: sums stay finite in either unit."""
+    from picolm_b200 import ops
+    n, scale = 2500, hd ** -0.5
+    s = Setup([n], G, hd, seed=hd).fill([n], G, hd)
+    for i in range(s.table.shape[1]):
+        s.vs[int(s.table[0, i])] = 2.0 ** (40 if i % 2 else low)
+    s.device()
+    for size in (0.0, 1.0):
+        q = (torch.randn((new, H, hd), generator=s.g) * size).bfloat16()
+        pos = [n - new + t for t in range(new)]
+        if new == 1:
+            outs = [ops.attention_kv8_decode(q.to(DEV), s.dk, s.dv, s.dks, s.dvs, i32(pos), i32([0]), s.dt, n, G, scale, n_splits=k) for k in (None, 0, 1, 8)]
+        else:
+            outs = [ops.attention_kv8_prefill(q.to(DEV), s.dk, s.dv, s.dks, s.dvs, i32([0, new]), i32([n]), s.dt, new, n, G, scale, **more)
+                    for more in (dict(), dict(keep_first=1, window=2 * n))]
+        for got in outs:
+            check(got, s, q, [(t, pos[t]) for t in sorted({0, new // 2, new - 1})], G, scale, 3)
